@@ -106,8 +106,11 @@ def _pkg():
 
 
 class _Shared:
-    def __init__(self, ptr, shape, kind):
-        self.__cuda_array_interface__ = {"data": (ptr, False), "shape": shape, "typestr": kind, "version": 3}
+    """An array's memory for torch; the tensor keeps the array alive."""
+
+    def __init__(self, array, shape, kind):
+        self.array = array
+        self.__cuda_array_interface__ = {"data": (array.ptr, False), "shape": shape, "typestr": kind, "version": 3}
 
 
 def _keep(s, name, value):
@@ -119,7 +122,7 @@ def _keep(s, name, value):
                  torch.int8: ("|i1", np.int8), torch.uint8: ("|u1", np.uint8), torch.int32: ("<i4", np.int32)}
         kind, dtype = kinds[t.dtype]
         a = p.ROCArray(dtype, tuple(reversed(t.shape)))
-        u = torch.as_tensor(_Shared(a.ptr, tuple(t.shape), kind), device=DEVICE).view(t.dtype)
+        u = torch.as_tensor(_Shared(a, tuple(t.shape), kind), device=DEVICE).view(t.dtype)
         u.copy_(t)
         s["array"][name] = a
         t = u
