@@ -24,6 +24,11 @@ from .accumulate import accumulate_, accumulate, cumsum, cumprod
 from .accumulate import prepared as accumulate_prepared
 from .sorting import sort_, sort, sortperm_, sortperm
 from .indexing import findall, getindex, getindex_mask, getindex_mask_dim, reverse, reverse_
+from .quantization import Quantized8, quantize_, quantize, dequantize_, dequantize
+from .normalization import layernorm_, layernorm, layernorm_backward_, layernorm_backward
+from .activation import activation_, activation, activation_backward_
+from .rotary import RotaryPlan, rotary_plan, rotary_
+from .kvcache import QuantizedCache, quantized_cache, cache_write_, cache_read_
 from . import random
 from . import graph
 from .graph import Graph, GraphExec, capture, instantiate, launch, update, is_capturing, captured

@@ -149,6 +149,15 @@ SIGNATURES = {
     "b200_compact": [_vp, _P(Tensor), _P(Tensor), _P(Tensor), _P(Tensor)],
     "b200_reverse": [_vp, _P(Tensor), _P(Tensor), C.c_uint32],
     "b200_gather": [_vp, _P(Tensor), _P(Tensor), _P(Tensor)],
+    "b200_layernorm": [_vp, _vp, _vp, _i32, _vp, _vp, C.c_double, _vp, _vp, _vp, _vp],
+    "b200_layernorm_backward": [_vp, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp],
+    "b200_quantize": [_vp, _vp, _vp, _vp],
+    "b200_dequantize": [_vp, _vp, _vp, _vp],
+    "b200_activation": [_vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
+    "b200_activation_backward": [_vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
+    "b200_rotary": [_vp, _vp, _vp, _vp, _vp, _i32, C.c_double, _i32],
+    "b200_cache_write": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, C.c_double],
+    "b200_cache_read": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
     "b200_graph_capture_begin": [_vp, C.c_int32],
     "b200_graph_capture_end": [_vp, _P(_vp)],
     "b200_stream_is_capturing": [_vp, _P(C.c_int32)],

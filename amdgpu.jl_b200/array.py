@@ -26,11 +26,12 @@ class _Managed:
     stream may still be using it (``dirty``).  An operation on another stream first takes the
     buffer over (:meth:`take_ownership`), and the stream-ordered free goes to the last owner."""
 
-    __slots__ = ("ptr", "nbytes", "stream", "dirty", "freed", "cached", "_lock", "__weakref__")
+    __slots__ = ("ptr", "nbytes", "device", "stream", "dirty", "freed", "cached", "_lock", "__weakref__")
 
     def __init__(self, nbytes: int, stream: Stream):
         self.ptr, self.freed = 0, True          # a failed allocation must leave a harmless object
         self.nbytes = nbytes
+        self.device = stream.device             # where the memory lies, whichever stream uses it
         self.stream = stream
         self.dirty = True
         self._lock = threading.Lock()
@@ -93,6 +94,16 @@ def with_managed(stream: Stream, *arrays) -> Stream:
     reads or writes is handed to the launch stream before the launch.  Returns `stream`."""
     for a in arrays:
         if a is not None:
+            a.buf.take_ownership(stream)
+    return stream
+
+
+def on_stream(stream: Stream, *arrays) -> Stream:
+    """:func:`with_managed` for operators that refuse arrays of another device than the stream's."""
+    for a in arrays:
+        if a is not None:
+            if a.buf.device != stream.device:
+                raise ValueError(f"an array of device {a.buf.device} cannot be used on a stream of device {stream.device}")
             a.buf.take_ownership(stream)
     return stream
 
@@ -172,6 +183,17 @@ class ROCArray:
             t.shape[i] = d
             t.stride[i] = s
         return t
+
+    def _ref(self):
+        """Reference to a descriptor that is made once: pointer, dims and strides never change.  For
+        the row operators, whose calls carry up to a dozen arrays."""
+        if self.buf.freed:
+            raise RuntimeError("use of a ROCArray after unsafe_free!")
+        try:
+            return self._desc
+        except AttributeError:
+            self._desc = C.byref(self.tensor())
+            return self._desc
 
     # ---- construction / conversion
     @classmethod

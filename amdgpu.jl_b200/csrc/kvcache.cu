@@ -1,0 +1,343 @@
+// Key/value cache held in 8 bits, in pages: new tokens are written (keys turned to their positions on
+// the way) and contexts are read back.  Scatter and gather of whole rows beside the element gather and
+// compaction of src/kernels/indexing.jl:8-36.
+//
+// A cache is four arrays: codes (head size, heads, page size, pages) and scale bytes (blocks of 32 of
+// a head, heads, page size, pages), for keys and for values.  Slots and pages are 1-based; slot s is
+// place (s-1) mod page size of page (s-1) div page size + 1.
+#include "rowops.cuh"
+
+namespace b200 {
+
+struct CacheSide {                              // keys or values
+    const void* x;                              // tokens: (head size, heads, tokens)
+    void* out;                                  // read back: (head size, heads, places, sequences)
+    uint8_t *q, *s;
+    int64_t xh, xt, oh, ol, ob;                 // element strides of tokens and of the read-back array
+    int64_t qh, qp, qn, sh, sp, sn;             // strides of codes and scale bytes: head, place, page
+    int32_t d, units;                           // units: vectors per token
+    FastDiv per_head;                           // vectors per head
+};
+struct CacheArgs {
+    CacheSide k, v;
+    const void *slots, *pos, *pages, *lengths;
+    const uint64_t* table;
+    uint32_t* owner;                            // per slot: highest token that claims it, plus one
+    int32_t* err;
+    int64_t tokens, nslots, npages, pl, pb, most, places, seqs;   // pl, pb: strides of the page table
+    int64_t islots, ipos, ilengths;                               // their strides
+    int32_t heads, page, rot, half, slots_wide, pos_wide, pages_wide, lengths_wide, e4m3, group;
+    float factor;
+};
+
+// Tokens above this many settle two claims on one slot through a table instead of by looking through
+// the later slots.
+constexpr int64_t kScanTokens = 2048;
+
+__global__ void __launch_bounds__(256)
+cache_claim_kernel(CacheArgs a) {
+    grid_dependency_wait();
+    const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (t >= a.tokens) return;
+    const int64_t slot = load_int(a.slots, a.slots_wide, t * a.islots);
+    if (slot >= 1 && slot <= a.nslots) atomicMax(a.owner + slot - 1, (uint32_t)t + 1u);
+}
+
+// V elements from place i of one head of a token, turned if `rot` reaches there.
+template <typename T, int V>
+__device__ __forceinline__ void load_turned(const T* x, int i, int rot, bool half, const float2* turn, float* v) {
+    unpack<T, V>(ld_raw_cached<T, V>(x + i), v);
+    if (i >= rot) return;
+    if (half) {
+        const int h = rot / 2;
+        const bool low = i < h;
+        float p[V];
+        unpack<T, V>(ld_raw_cached<T, V>(x + (low ? i + h : i - h)), p);
+        const float2* w = turn + (low ? i : i - h);
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = fmaf(v[j], w[j].x, (low ? -p[j] : p[j]) * w[j].y);
+    } else if constexpr (V == 1) {
+        const float p = Elem<T>::get(x[i ^ 1]);
+        const float2 w = turn[i / 2];
+        v[0] = fmaf(v[0], w.x, (i & 1 ? p : -p) * w.y);
+    } else {
+#pragma unroll
+        for (int j = 0; j < V / 2; ++j) {
+            const float2 w = turn[i / 2 + j];
+            const float x0 = v[2 * j], x1 = v[2 * j + 1];
+            v[2 * j] = fmaf(x0, w.x, -(x1 * w.y));
+            v[2 * j + 1] = fmaf(x1, w.x, x0 * w.y);
+        }
+    }
+}
+
+// `group` threads (whole warps) per token; the 32/V lanes of a block of 32 are neighbours.
+template <typename T, int V>
+__global__ void __launch_bounds__(256)
+cache_write_kernel(CacheArgs a) {
+    extern __shared__ float2 turns[];            // [tokens of the block][rot / 2] cosine, sine
+    __shared__ int lost[8];
+    grid_dependency_wait();
+    const int G = a.group, group = threadIdx.x / G, lane = threadIdx.x % G;
+    const int64_t t = (int64_t)blockIdx.x * (256 / G) + group;
+    const bool live = t < a.tokens;
+    float2* turn = turns + group * (a.rot / 2);
+    if (lane == 0) lost[group] = 0;
+    __syncthreads();
+    const int64_t slot = live ? load_int(a.slots, a.slots_wide, t * a.islots) : 0;
+    const bool ok = slot >= 1 && slot <= a.nslots;
+    if (live && !ok && slot != 0 && lane == 0) latch_error(a.err, B200_INVALID_ARG);
+    if (ok) {
+        // of several tokens with one slot the last is kept, as if they were written in turn
+        if (a.owner) {
+            if (lane == 0 && a.owner[slot - 1] != (uint32_t)t + 1u) lost[group] = 1;
+        } else {
+            for (int64_t j = t + 1 + lane; j < a.tokens; j += G)
+                if (load_int(a.slots, a.slots_wide, j * a.islots) == slot) lost[group] = 1;
+        }
+        if (a.rot) {
+            const uint64_t pos = (uint64_t)load_int(a.pos, a.pos_wide, t * a.ipos);
+            for (int i = lane; i < a.rot / 2; i += G) {
+                float s, c;
+                phase_sincos(pos * a.table[i], a.factor, s, c);
+                turn[i] = make_float2(c, s);
+            }
+        }
+    }
+    __syncthreads();
+    const bool write = ok && !lost[group];
+    const int64_t page = ok ? (slot - 1) / a.page : 0, place = ok ? (slot - 1) - page * a.page : 0;
+    for (int base = 0; base < a.k.units + a.v.units; base += G) {
+        int u = base + lane;
+        const bool key = u < a.k.units;
+        if (!key) u -= a.k.units;
+        const CacheSide& side = key ? a.k : a.v;
+        const bool some = write && u < side.units;
+        const int h = some ? (int)side.per_head.div((uint32_t)u) : 0;
+        const int i = some ? (u - h * (int)side.per_head.d) * V : 0;
+        const bool in = some && i < side.d;
+        float v[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = 0.f;
+        if (in) load_turned<T, V>(reinterpret_cast<const T*>(side.x) + t * side.xt + h * side.xh, i, key ? a.rot : 0, a.half, turn, v);
+        const uint32_t e = scale_byte(block_amax<V>(v), a.e4m3);
+        if (in) {
+            *reinterpret_cast<RawVec<uint8_t, V>*>(side.q + page * side.qn + place * side.qp + h * side.qh + i) = encode<V>(v, e, a.e4m3);
+            if (i % kBlock == 0) side.s[page * side.sn + place * side.sp + h * side.sh + i / kBlock] = (uint8_t)e;
+        }
+    }
+}
+
+template <typename T, int V>
+__global__ void __launch_bounds__(256)
+cache_read_kernel(CacheArgs a) {
+    grid_dependency_wait();
+    const int per_token = a.k.units + a.v.units;
+    const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t l = n / per_token;
+    for (int64_t b = blockIdx.y; b < a.seqs; b += gridDim.y) {
+        int64_t length = load_int(a.lengths, a.lengths_wide, b * a.ilengths);
+        const int64_t cap = min(a.places, a.most * a.page);
+        if (length < 0 || length > cap) {
+            if (n == 0) latch_error(a.err, B200_INVALID_ARG);
+            length = length < 0 ? 0 : cap;
+        }
+        if (l >= length) continue;
+        const int64_t pi = l / a.page, place = l - pi * a.page;
+        const int64_t page = load_int(a.pages, a.pages_wide, pi * a.pl + b * a.pb) - 1;
+        if (page < 0 || page >= a.npages) { latch_error(a.err, B200_INVALID_ARG); continue; }
+        int u = (int)(n - l * per_token);
+        const bool key = u < a.k.units;
+        if (!key) u -= a.k.units;
+        const CacheSide& side = key ? a.k : a.v;
+        const int h = (int)side.per_head.div((uint32_t)u);
+        const int i = (u - h * (int)side.per_head.d) * V;
+        float v[V];
+        decode_as<T, V>(ld_raw<uint8_t, V>(side.q + page * side.qn + place * side.qp + h * side.qh + i),
+                        side.s[page * side.sn + place * side.sp + h * side.sh + i / kBlock], a.e4m3, v);
+        st_raw<T, V>(reinterpret_cast<T*>(side.out) + b * side.ob + l * side.ol + h * side.oh + i, pack<T, V>(v));
+    }
+}
+
+// ---- host ---------------------------------------------------------------------------------------
+static int32_t cache_side(const b200_tensor* Q, const b200_tensor* S, const char* name, CacheSide* c) {
+    B200_TRY(check_codes(Q, S, name));
+    if (Q->ndim != 4) return fail(B200_INVALID_ARG, "%s: codes are (head size, heads, page size, pages)", name);
+    if ((Q->shape[0] > 1 && Q->stride[0] != 1) || (S->shape[0] > 1 && S->stride[0] != 1))
+        return fail(B200_UNSUPPORTED, "%s: the elements of a head must be neighbours", name);
+    c->q = (uint8_t*)Q->ptr; c->s = (uint8_t*)S->ptr;
+    c->d = (int32_t)Q->shape[0];
+    c->qh = Q->stride[1]; c->qp = Q->stride[2]; c->qn = Q->stride[3];
+    c->sh = S->stride[1]; c->sp = S->stride[2]; c->sn = S->stride[3];
+    return B200_OK;
+}
+static int32_t cache_pair(const b200_tensor* KQ, const b200_tensor* KS, const b200_tensor* VQ, const b200_tensor* VS, CacheArgs* a) {
+    B200_TRY(cache_side(KQ, KS, "cache keys", &a->k));
+    B200_TRY(cache_side(VQ, VS, "cache values", &a->v));
+    for (int k = 1; k < 4; ++k)
+        if (KQ->shape[k] != VQ->shape[k]) return fail(B200_INVALID_ARG, "cache: keys and values differ in heads, page size or pages");
+    if (KQ->dtype != VQ->dtype) return fail(B200_INVALID_ARG, "cache: keys and values differ in format");
+    if (KQ->shape[0] > 8192 || VQ->shape[0] > 8192 || KQ->shape[1] > 65536 || KQ->shape[2] > 0x3fffffff)
+        return fail(B200_TOO_LARGE, "cache: heads of at most 8192 elements, 65536 heads, pages of at most 2^30-1 places");
+    a->heads = (int32_t)KQ->shape[1];
+    a->page = (int32_t)KQ->shape[2];
+    a->npages = KQ->shape[3];
+    a->nslots = KQ->shape[2] * KQ->shape[3];
+    a->e4m3 = KQ->dtype == B200_U8;
+    return B200_OK;
+}
+static int32_t cache_rows(const b200_tensor* t, const b200_tensor* Q, int ndim, const char* name, int32_t* dtype) {
+    B200_TRY(check_tensor(t, name));
+    if (t->ndim != ndim || t->shape[0] != Q->shape[0] || t->shape[1] != Q->shape[1])
+        return fail(B200_INVALID_ARG, "%s: differs in head size or heads from the cache", name);
+    if (!is_row_type(t->dtype)) return fail(B200_UNSUPPORTED, "%s: Float16, BFloat16 or Float32", name);
+    if (*dtype >= 0 && *dtype != t->dtype) return fail(B200_INVALID_ARG, "%s: keys and values differ in element type", name);
+    if (t->shape[0] > 1 && t->stride[0] != 1) return fail(B200_UNSUPPORTED, "%s: the elements of a head must be neighbours", name);
+    *dtype = t->dtype;
+    return B200_OK;
+}
+static int32_t index_vector(const b200_tensor* t, const char* name, int64_t n, const void** p, int64_t* stride, int32_t* wide) {
+    B200_TRY(check_tensor(t, name));
+    if (!is_index_type(t->dtype)) return fail(B200_UNSUPPORTED, "%s: must be Int32 or Int64", name);
+    if (t->ndim != 1 || t->shape[0] != n) return fail(B200_INVALID_ARG, "%s: needs %lld entries", name, (long long)n);
+    *p = t->ptr; *stride = t->stride[0]; *wide = t->dtype == B200_I64;
+    return B200_OK;
+}
+static bool multiple_strides(const b200_tensor* t, int64_t v, size_t bytes) {
+    for (int k = 1; k < t->ndim; ++k) if (t->shape[k] > 1 && t->stride[k] % v) return false;
+    return reinterpret_cast<uintptr_t>(t->ptr) % bytes == 0;
+}
+static int32_t no_overlap(const b200_tensor* t, const char* name) {
+    if (tensor_numel(t) == 0) return B200_OK;
+    for (int k = 1; k < t->ndim; ++k)
+        if (t->shape[k] > 1 && t->stride[k] < t->shape[0] && t->stride[k] > -t->shape[0]) return fail(B200_INVALID_ARG, "%s: heads overlap", name);
+    return B200_OK;
+}
+
+template <typename F>
+static cudaError_t by_row_type(int32_t dtype, int v, F f) {
+    switch (dtype) {
+        case B200_F16: return v == 1 ? f(__half{}, std::integral_constant<int, 1>{}) : f(__half{}, std::integral_constant<int, 8>{});
+        case B200_BF16: return v == 1 ? f(__nv_bfloat16{}, std::integral_constant<int, 1>{}) : f(__nv_bfloat16{}, std::integral_constant<int, 8>{});
+        default: return v == 1 ? f(float{}, std::integral_constant<int, 1>{}) : f(float{}, std::integral_constant<int, 4>{});
+    }
+}
+
+}  // namespace b200
+
+using namespace b200;
+
+extern "C" int32_t b200_cache_write(b200_stream_t st, const b200_tensor* KQ, const b200_tensor* KS, const b200_tensor* VQ,
+                                    const b200_tensor* VS, const b200_tensor* K, const b200_tensor* V, const b200_tensor* slots,
+                                    const b200_tensor* positions, const b200_tensor* table, int32_t layout, double factor) {
+    CacheArgs a{};
+    B200_TRY(cache_pair(KQ, KS, VQ, VS, &a));
+    B200_TRY(no_overlap(KQ, "cache keys"));
+    B200_TRY(no_overlap(VQ, "cache values"));
+    int32_t dtype = -1;
+    B200_TRY(cache_rows(K, KQ, 3, "cache write keys", &dtype));
+    B200_TRY(cache_rows(V, VQ, 3, "cache write values", &dtype));
+    if (K->shape[2] != V->shape[2]) return fail(B200_INVALID_ARG, "cache write: keys and values differ in tokens");
+    a.tokens = K->shape[2];
+    B200_TRY(index_vector(slots, "cache write slots", a.tokens, &a.slots, &a.islots, &a.slots_wide));
+    if ((positions != nullptr) != (table != nullptr)) return fail(B200_INVALID_ARG, "cache write: positions and their table belong together");
+    if (table) {
+        if (layout != kRotaryHalf && layout != kRotaryInterleaved) return fail(B200_UNSUPPORTED, "cache write: layout half (0) or interleaved (1)");
+        B200_TRY(check_tensor(table, "rotary table"));
+        if (table->dtype != B200_U64 || !tensor_is_contiguous(table)) return fail(B200_UNSUPPORTED, "cache write: the table must be dense UInt64");
+        if (2 * tensor_numel(table) > K->shape[0]) return fail(B200_INVALID_ARG, "cache write: the table turns more elements than a head has");
+        B200_TRY(index_vector(positions, "cache write positions", a.tokens, &a.pos, &a.ipos, &a.pos_wide));
+        a.rot = (int32_t)(2 * tensor_numel(table));
+        a.table = reinterpret_cast<const uint64_t*>(table->ptr);
+        a.half = layout == kRotaryHalf;
+        a.factor = (float)factor;
+    }
+    B200_TRY(enter(st));
+    StreamGuard guard(st);
+    if (a.tokens == 0 || a.heads == 0 || (a.k.d == 0 && a.v.d == 0)) return B200_OK;
+    if (a.tokens > 0x7ffffff0) return fail(B200_TOO_LARGE, "cache write: at most 2^31-16 tokens");
+    if (a.page == 0) a.page = 1;                                    // no slot is valid then
+    a.k.x = K->ptr; a.k.xh = K->stride[1]; a.k.xt = K->stride[2];
+    a.v.x = V->ptr; a.v.xh = V->stride[1]; a.v.xt = V->stride[2];
+    a.err = device_error_word(st->dev);
+    const int fv = dtype == B200_F32 ? 4 : 8;
+    const bool vec = a.k.d % fv == 0 && a.v.d % fv == 0 && multiple_strides(K, fv, 16) && multiple_strides(V, fv, 16) &&
+                     multiple_strides(KQ, fv, (size_t)fv) && multiple_strides(VQ, fv, (size_t)fv) && (a.half ? a.rot / 2 : a.rot) % fv == 0;
+    const int v = vec ? fv : 1;
+    for (CacheSide* s : {&a.k, &a.v}) {
+        const int per = (int)(row_blocks(s->d) * (kBlock / v));
+        s->units = per * a.heads;
+        s->per_head = FastDiv((uint32_t)per);
+    }
+    a.group = 32;
+    while (a.group < 256 && a.group < a.k.units + a.v.units) a.group *= 2;
+    const int per_block = 256 / a.group;
+    void* temp = nullptr;
+    if (a.tokens > kScanTokens && a.nslots > 0) {
+        cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+        B200_CUDA(cudaStreamIsCapturing(st->s, &cap));
+        void* p = nullptr;
+        // a graph gets a table of its own (graphs captured on one stream may run side by side)
+        if (cap == cudaStreamCaptureStatusNone) B200_TRY(scratch(st, (size_t)a.nslots * 4, &p));
+        else { B200_TRY(b200_malloc_async(&temp, (size_t)a.nslots * 4, st)); p = temp; }
+        a.owner = reinterpret_cast<uint32_t*>(p);
+        B200_CUDA(cudaMemsetAsync(p, 0, (size_t)a.nslots * 4, st->s));
+        B200_CUDA(launch_overlapped(cache_claim_kernel, (unsigned)((a.tokens + 255) / 256), 256u, 0, st->s, a));
+    }
+    const size_t smem = (size_t)per_block * (a.rot / 2) * sizeof(float2);
+    const unsigned grid = (unsigned)((a.tokens + per_block - 1) / per_block);
+    B200_CUDA(by_row_type(dtype, v, [&](auto t, auto w) {
+        return launch_overlapped(cache_write_kernel<decltype(t), decltype(w)::value>, grid, 256u, smem, st->s, a);
+    }));
+    if (temp) B200_TRY(b200_free_async(temp, st));
+    return finish(st, "b200_cache_write");
+}
+
+extern "C" int32_t b200_cache_read(b200_stream_t st, const b200_tensor* K, const b200_tensor* V, const b200_tensor* KQ, const b200_tensor* KS,
+                                   const b200_tensor* VQ, const b200_tensor* VS, const b200_tensor* pages, const b200_tensor* lengths) {
+    CacheArgs a{};
+    B200_TRY(cache_pair(KQ, KS, VQ, VS, &a));
+    int32_t dtype = -1;
+    B200_TRY(cache_rows(K, KQ, 4, "cache read keys", &dtype));
+    B200_TRY(cache_rows(V, VQ, 4, "cache read values", &dtype));
+    B200_TRY(no_overlap(K, "cache read keys"));
+    B200_TRY(no_overlap(V, "cache read values"));
+    if (K->shape[2] != V->shape[2] || K->shape[3] != V->shape[3]) return fail(B200_INVALID_ARG, "cache read: keys and values differ in places or sequences");
+    a.places = K->shape[2];
+    a.seqs = K->shape[3];
+    B200_TRY(check_tensor(pages, "cache read pages"));
+    if (!is_index_type(pages->dtype)) return fail(B200_UNSUPPORTED, "cache read: pages must be Int32 or Int64");
+    if (pages->ndim != 2 || pages->shape[1] != a.seqs) return fail(B200_INVALID_ARG, "cache read: the page table is (pages of a sequence, sequences)");
+    a.pages = pages->ptr; a.pl = pages->stride[0]; a.pb = pages->stride[1]; a.most = pages->shape[0]; a.pages_wide = pages->dtype == B200_I64;
+    B200_TRY(index_vector(lengths, "cache read lengths", a.seqs, &a.lengths, &a.ilengths, &a.lengths_wide));
+    B200_TRY(enter(st));
+    StreamGuard guard(st);
+    if (a.seqs == 0 || a.heads == 0 || (a.k.d == 0 && a.v.d == 0)) return B200_OK;
+    if (a.page == 0) { a.page = 1; a.most = 0; }                    // no place holds a token
+    a.k.out = K->ptr; a.k.oh = K->stride[1]; a.k.ol = K->stride[2]; a.k.ob = K->stride[3];
+    a.v.out = V->ptr; a.v.oh = V->stride[1]; a.v.ol = V->stride[2]; a.v.ob = V->stride[3];
+    a.err = device_error_word(st->dev);
+    const int fv = dtype == B200_F32 ? 4 : 8;
+    const bool vec = a.k.d % fv == 0 && a.v.d % fv == 0 && multiple_strides(K, fv, 16) && multiple_strides(V, fv, 16) &&
+                     multiple_strides(KQ, fv, (size_t)fv) && multiple_strides(VQ, fv, (size_t)fv);
+    const int v = vec ? fv : 1;
+    for (CacheSide* s : {&a.k, &a.v}) {
+        s->units = s->d / v * a.heads;
+        s->per_head = FastDiv((uint32_t)(s->d / v));
+    }
+    const int64_t n = a.places * (a.k.units + a.v.units);
+    const int64_t bx = n > 0 ? (n + 255) / 256 : 1;                 // one block at least looks at the lengths
+    if (bx > 0x7fffffff) return fail(B200_TOO_LARGE, "cache read: too many places for one call");
+    const dim3 grid((unsigned)bx, (unsigned)(a.seqs < 65535 ? a.seqs : 65535));
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(256);
+    cfg.stream = st->s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = overlap_launches_enabled() ? 1 : 0;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    B200_CUDA(by_row_type(dtype, v, [&](auto t, auto w) { return cudaLaunchKernelEx(&cfg, cache_read_kernel<decltype(t), decltype(w)::value>, a); }));
+    return finish(st, "b200_cache_read");
+}

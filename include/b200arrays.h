@@ -280,6 +280,81 @@ int32_t b200_reverse(b200_stream_t st, const b200_tensor* y, const b200_tensor* 
 int32_t b200_fill_random(b200_stream_t st, const b200_tensor* out, int32_t dist, uint64_t seed,
                          uint64_t stream_id, uint64_t first_index, int64_t lo, int64_t hi);
 
+/* ---- row operators ------------------------------------------------------------------------- */
+/* The memory-bound operators around the matrix products of a transformer block.  The reference
+ * composes them from mapreduce and broadcast calls (src/kernels/mapreduce.jl:86-173,
+ * src/broadcast.jl:3-30); here each is one pass over its rows.  Element types Float16, BFloat16 and
+ * Float32; sums, moments, angles and products are held in binary32 or wider and rounded once on the
+ * store.  A destination may be the same array as an operand of its own type; any other overlap is
+ * the caller's error.
+ *
+ * 8-bit form of an array: `Q` has its shape, Int8 codes or UInt8 bytes of e4m3 (1-4-3 bits, no
+ * infinities); `S` (UInt8) has one scale byte e per block of 32 elements of the first dimension, the
+ * last block of a row may be shorter.  The scale is 2^(e-127), the smallest such power (e >= 0) that
+ * brings the block's largest magnitude to 127 (Int8) or 448 (e4m3); a code is the value over the
+ * scale, rounded to nearest even.  A block that holds an infinity or a NaN has e = 255 and reads
+ * back as NaN.  Read back into a type too narrow for a value, that value becomes the type's largest. */
+
+/* Layer norm: the first `lead` dimensions of X are one row, normalised together.
+ * Y = (X - m) r gamma + beta, m = mean, r = 1/sqrt(variance + eps) of each row.  gamma and beta hold
+ * one value per element of a row, both Float32 or both of X's type; either may be NULL.  mean, rstd:
+ * NULL, or Float32, one per row, for the gradient.  Q, S: NULL, or receive the rows (X - m) r in
+ * 8 bits (lead must be 1), which the gradient takes instead of X and mean.  Rows are dense and may be
+ * any one distance apart. */
+int32_t b200_layernorm(b200_stream_t st, const b200_tensor* Y, const b200_tensor* X, int32_t lead,
+                       const b200_tensor* gamma, const b200_tensor* beta, double eps,
+                       const b200_tensor* mean, const b200_tensor* rstd,
+                       const b200_tensor* Q, const b200_tensor* S);
+/* Its gradient.  Either X with mean and rstd, or Q, S and rstd.  dX, dgamma, dbeta: any may be NULL,
+ * not all; dgamma and dbeta have gamma's element type and are overwritten; the order of their sums
+ * depends on the shapes and the device only, so repeated calls give the same bits. */
+int32_t b200_layernorm_backward(b200_stream_t st, const b200_tensor* dX, const b200_tensor* dgamma,
+                                const b200_tensor* dbeta, const b200_tensor* dY, int32_t lead,
+                                const b200_tensor* X, const b200_tensor* Q, const b200_tensor* S,
+                                const b200_tensor* gamma, const b200_tensor* mean, const b200_tensor* rstd);
+
+/* Rows to 8 bits and back; X may have rows any one distance apart, Q and S are dense. */
+int32_t b200_quantize(b200_stream_t st, const b200_tensor* Q, const b200_tensor* S, const b200_tensor* X);
+int32_t b200_dequantize(b200_stream_t st, const b200_tensor* X, const b200_tensor* Q, const b200_tensor* S);
+/* Y = f(A), or f(A) B with a gate B; act 0: silu, 1: gelu (tanh form).  QA, SA and QB, SB: NULL, or
+ * receive A and B in 8 bits for the gradient. */
+int32_t b200_activation(b200_stream_t st, int32_t act, const b200_tensor* Y, const b200_tensor* A,
+                        const b200_tensor* B, const b200_tensor* QA, const b200_tensor* SA,
+                        const b200_tensor* QB, const b200_tensor* SB);
+/* dA = dY f'(A) [B], dB = dY f(A); A and B as arrays, or both out of 8 bits.  dB NULL: no gate. */
+int32_t b200_activation_backward(b200_stream_t st, int32_t act, const b200_tensor* dA, const b200_tensor* dB,
+                                 const b200_tensor* dY, const b200_tensor* A, const b200_tensor* B,
+                                 const b200_tensor* QA, const b200_tensor* SA,
+                                 const b200_tensor* QB, const b200_tensor* SB);
+
+/* Rotary positions: X is (head size, heads, tokens) or (head size, heads, tokens, batch), any strides
+ * above the first dimension.  positions (Int32 or Int64, may be negative): one per token, or per
+ * token and batch entry.  table (UInt64): angle per position of each pair, in 2^-64 turns; its length
+ * is half the number of elements turned at the front of a head, the rest pass through.  layout 0:
+ * pairs (i, i + rot/2), 1: (2i, 2i+1).  factor scales cosine and sine.  adjoint != 0 turns backwards,
+ * which is the gradient. */
+int32_t b200_rotary(b200_stream_t st, const b200_tensor* Y, const b200_tensor* X,
+                    const b200_tensor* positions, const b200_tensor* table, int32_t layout,
+                    double factor, int32_t adjoint);
+
+/* Key/value cache in 8 bits.  KQ, VQ: codes (head size, heads, page size, pages), KS, VS: scale bytes
+ * (blocks of 32 of a head, heads, page size, pages), any strides above the first dimension.
+ * Write: K, V are (head size, heads, tokens); slots (Int32 or Int64) holds one 1-based slot per token,
+ * page-major; slot 0 leaves the token out; of several tokens with one slot the last is kept.  A slot
+ * outside the cache latches B200_INVALID_ARG, reported by the next b200_stream_sync, and writes
+ * nothing.  positions, table, layout, factor: NULL, or turn the keys on the way (b200_rotary). */
+int32_t b200_cache_write(b200_stream_t st, const b200_tensor* KQ, const b200_tensor* KS,
+                         const b200_tensor* VQ, const b200_tensor* VS, const b200_tensor* K,
+                         const b200_tensor* V, const b200_tensor* slots, const b200_tensor* positions,
+                         const b200_tensor* table, int32_t layout, double factor);
+/* Read: K, V are (head size, heads, places, sequences); place l of sequence b comes from page
+ * pages[l div page size, b] (1-based).  Places from lengths[b] on are left as they were.  A length
+ * that is negative or passes the places or the page table, or a page outside the cache, latches
+ * B200_INVALID_ARG; what is in range is read. */
+int32_t b200_cache_read(b200_stream_t st, const b200_tensor* K, const b200_tensor* V,
+                        const b200_tensor* KQ, const b200_tensor* KS, const b200_tensor* VQ,
+                        const b200_tensor* VS, const b200_tensor* pages, const b200_tensor* lengths);
+
 /* ---- graphs (replaces src/hip/graph.jl:16-168: capture, instantiate, launch, update,
  * is_capturing) --------------------------------------------------------------------------- */
 /* Every operator above can be captured.  An operator that needs more stream scratch than the
