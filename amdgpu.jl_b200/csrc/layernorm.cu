@@ -21,6 +21,8 @@ struct NormArgs {
     uint8_t *q, *s;                     // codes and scale bytes of the normalised rows
     float *partial;                     // gradient: [block][2][d] sums of dy*h and dy
     int64_t ldx, ldy, lddy, rows, d, blocks;
+    // ring kernels: rows from one of a group's to its next, and that many rows of each array in elements
+    int64_t step, x_step, y_step, dy_step, q_step;
     float eps;
     int32_t gamma_f32, e4m3, group;     // group: threads per row, a power of two
 };
@@ -41,10 +43,10 @@ __device__ __forceinline__ float lane_sum(float v, int width) {
     return v;
 }
 
-// ---- rows in registers --------------------------------------------------------------------------
-// `group` threads hold one row, NV vectors of V elements each, so a row is read once; a block of
-// kNormThreads (or one group, if that is larger) works on several rows side by side and walks over
-// the rows with the grid's stride.  gamma and beta stay in registers.
+// ---- rows of any alignment ------------------------------------------------------------------------
+// `group` threads hold one row, element by element, so a row is read once; a block of kNormThreads (or one
+// group, if that is larger) works on several rows side by side and walks over the rows with the grid's
+// stride.
 //
 // Moments in one exchange: every warp takes the mean of its share and the squares about that mean;
 // the shares combine as M2 = sum M2_w + n_w (mean_w - mean)^2 (Chan, Golub and LeVeque 1983), which
@@ -260,26 +262,464 @@ norm_backward_kernel(NormArgs a) {
     }
 }
 
-// Sums the blocks' partials: 32 columns per block, eight strands of blocks, joined in a fixed order.
-__global__ void __launch_bounds__(256)
-norm_fold_kernel(const float* partial, int64_t nblocks, int64_t d, void* dgamma, void* dbeta, int32_t dtype) {
-    __shared__ float part[8][33];
-    grid_dependency_wait();
-    const int lane = threadIdx.x % 32, strand = threadIdx.x / 32;
-    const int64_t c = (int64_t)blockIdx.x * 32 + lane;      // over [dgamma | dbeta]
-    float sum = 0.f;
-    if (c < 2 * d) for (int64_t b = strand; b < nblocks; b += 8) sum += partial[b * 2 * d + c];
-    part[strand][lane] = sum;
-    __syncthreads();
-    if (strand != 0 || c >= 2 * d) return;
+// ---- rows through a ring in shared memory -----------------------------------------------------------
+// Aligned rows of whole vectors.  `group` threads hold a row, E elements each; a block has as many groups
+// as fit and every group walks over the rows with the grid's stride, STAGES - 1 rows ahead of its own work.
+// A thread copies its own vectors (cp.async, 16 bytes) into its own places of the ring and reads only
+// those, so the ring needs no barrier: a thread waits for its own copies.  Groups run on their own, with a
+// hardware barrier each for their sums, so that some load while others compute and store.
+//
+// With the loads out of the way these kernels are bound by instruction issue, not by HBM: arithmetic goes
+// in pairs (F2), a thread has as many columns as its registers hold, and nothing is predicated but the
+// copies and stores (vectors beyond a row read as zeros).  One B200, 16384 x 4096 BFloat16: forward 48 us
+// (5.5 TB/s), with the 8-bit rows written as well 61 us, gradient 69 us (5.8 TB/s), from the 8-bit rows
+// 72 us; waiting for each row in turn the gradient takes 120 us.  A register spilled inside the loop costs
+// more than a second pass over it (20 bytes: 69 -> 84 us).
+
+enum { kAsIs = 0, kInt8 = 1, kE4M3 = 2 };   // form of the rows kept for the gradient
+
+struct GroupBarrier {
+    int id, threads;
+    __device__ __forceinline__ void sync() const { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+};
+// What a thread of a ring kernel knows about its place and its rows: row + i * step for i < mine.
+struct RingPlace {
+    int group, t, warps, warp, lane, width, mine, walk;
+    int64_t row;
+    GroupBarrier bar;
+    __device__ __forceinline__ RingPlace(int G, int64_t rows, int64_t step) {
+        const int per_block = blockDim.x / G;
+        group = threadIdx.x / G;
+        t = threadIdx.x % G;
+        warps = G / 32; warp = t / 32; lane = t % 32;
+        width = G < 32 ? G : 32;
+        bar = GroupBarrier{group + 1, G};
+        row = (int64_t)blockIdx.x * per_block + group;
+        mine = row < rows ? (int)((rows - row + step - 1) / step) : 0;
+        // exchanges take whole warps: groups that share one walk as often as its first, which has most rows
+        walk = __shfl_sync(0xffffffffu, mine, 0);
+    }
+};
+// Places for the warps' sums: zero beyond the group's warps, whole vectors for the reader.
+constexpr int kShare = 16;
+// Sum over a group.
+__device__ __forceinline__ float group_sum(float v, const RingPlace& p, float* share) {
+    v = lane_sum(v, p.width);
+    if (p.warps <= 1) return v;
+    if (p.lane == 0) share[p.warp] = v;
+    p.bar.sync();
+    const float4* q = reinterpret_cast<const float4*>(share);
+    float4 a = q[0], b = q[1];
+    v = ((a.x + a.y) + (a.z + a.w)) + ((b.x + b.y) + (b.z + b.w));
+    if (p.warps > 8) {
+        a = q[2]; b = q[3];
+        v += ((a.x + a.y) + (a.z + a.w)) + ((b.x + b.y) + (b.z + b.w));
+    }
+    return v;
+}
+// Two sums at once: after the first exchange one half of the lanes carries each.
+__device__ __forceinline__ float2 group_sum2(float a, float b, const RingPlace& p, float2* share) {
+    if (p.width < 32) {
+        a = lane_sum(a, p.width);
+        return make_float2(a, lane_sum(b, p.width));
+    }
+    const bool upper = p.lane & 16;
+    float v = (upper ? b : a) + __shfl_xor_sync(0xffffffffu, upper ? a : b, 16);
 #pragma unroll
-    for (int k = 1; k < 8; ++k) sum += part[k][lane];
-    void* out = c < d ? dgamma : dbeta;
+    for (int o = 8; o > 0; o /= 2) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (p.warps <= 1) {
+        const float other = __shfl_xor_sync(0xffffffffu, v, 16);
+        return upper ? make_float2(other, v) : make_float2(v, other);
+    }
+    if ((p.lane & 15) == 0) reinterpret_cast<float*>(share + p.warp)[upper] = v;
+    p.bar.sync();
+    const ulonglong2* q = reinterpret_cast<const ulonglong2*>(share);
+    const ulonglong2 u0 = q[0], u1 = q[1], u2 = q[2], u3 = q[3];
+    F2 sum = f2_add(f2_add(f2_add(u0.x, u0.y), f2_add(u1.x, u1.y)), f2_add(f2_add(u2.x, u2.y), f2_add(u3.x, u3.y)));
+    if (p.warps > 8) {
+#pragma unroll
+        for (int w = 4; w < 8; ++w) { const ulonglong2 u = q[w]; sum = f2_add(sum, f2_add(u.x, u.y)); }
+    }
+    return f2_parts(sum);
+}
+template <int BYTES>
+__device__ __forceinline__ void ring_copy(void* dst, const void* src) {
+    const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(src) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(d), "l"(src), "n"(BYTES) : "memory");
+}
+template <typename T, int V, int NV>
+__device__ __forceinline__ void load_params2(const NormArgs& a, const void* p, int t, int nvec, float missing, F2* out) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        const int vi = t + k * a.group;
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) out[k * V / 2 + i] = f2(missing);
+        if (!p || vi >= nvec) continue;
+        if (a.gamma_f32) {
+#pragma unroll
+            for (int i = 0; i < V / 4; ++i) {
+                const float* f = reinterpret_cast<const float*>(p) + (int64_t)vi * V + 4 * i;
+                out[k * V / 2 + 2 * i] = f2(f[0], f[1]);
+                out[k * V / 2 + 2 * i + 1] = f2(f[2], f[3]);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) {
+                const T* f = reinterpret_cast<const T*>(p) + (int64_t)vi * V + 2 * i;
+                out[k * V / 2 + i] = f2(Elem<T>::get(f[0]), Elem<T>::get(f[1]));
+            }
+        }
+    }
+}
+
+// Two passes over the row in registers: the mean first, then the squares about it.
+template <typename T, int E, int STAGES, int THREADS, int KEEP>
+__global__ void __launch_bounds__(THREADS)
+norm_forward_ring_kernel(NormArgs a) {
+    constexpr int V = 16 / (int)sizeof(T), NV = E / V, SLOT = NV * THREADS;
+    extern __shared__ uint4 ring[];                       // [stage][vector][thread]
+    __shared__ __align__(16) float shares[THREADS / 64][4][kShare];
+    for (int i = threadIdx.x; i < (int)(sizeof(shares) / 4); i += blockDim.x) (&shares[0][0][0])[i] = 0.f;
+    __syncthreads();
+    grid_dependency_wait();
+    const RingPlace p(a.group, a.rows, a.step);
+    const int G = a.group, t = p.t, nvec = (int)(a.d / V);
+    bool in[NV];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) in[k] = t + k * G < nvec;
+    const T* src = reinterpret_cast<const T*>(a.x) + p.row * a.ldx + (int64_t)t * V;      // next row to fetch
+    T* dst = reinterpret_cast<T*>(a.y) + p.row * a.ldy + (int64_t)t * V;
+    uint4* own = ring + threadIdx.x;
+    int to_fetch = p.mine;
+    auto fetch = [&](int slot) {
+        if (to_fetch > 0) {
+#pragma unroll
+            for (int k = 0; k < NV; ++k)
+                if (in[k]) ring_copy<16>(own + slot + k * THREADS, src + k * G * V);
+        }
+        --to_fetch;
+        src += a.x_step;
+        cp_async_commit();
+    };
+    // places that no copy fills: the vectors beyond the row read as zeros
+#pragma unroll
+    for (int s = 0; s < STAGES; ++s) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) if (!in[k]) own[s * SLOT + k * THREADS] = make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; ++s) fetch(s * SLOT);
+    F2 gm[E / 2], bt[E / 2];
+    load_params2<T, V, NV>(a, a.gamma, t, nvec, 1.f, gm);
+    load_params2<T, V, NV>(a, a.beta, t, nvec, 0.f, bt);
+    const float per_d = 1.f / (float)a.d;
+    int slot = 0, free_slot = (STAGES - 1) * SLOT;
+    float* share = &shares[p.warps > 1 ? p.group : 0][0][0];
+    int64_t row = p.row;
+    for (int it = 0; it < p.walk; ++it, row += a.step) {
+        const bool live = it < p.mine;
+        cp_async_wait<STAGES - 2>();
+        F2 v[E / 2];
+        F2 sum2 = f2(0.f);
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            unpack2<T, V>(own[slot + k * THREADS], v + k * V / 2);
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) sum2 = f2_add(sum2, v[k * V / 2 + i]);
+        }
+        fetch(free_slot);
+        free_slot = slot;
+        slot = slot == (STAGES - 1) * SLOT ? 0 : slot + SLOT;
+        const float mean = group_sum(f2_total(sum2), p, share) * per_d;
+        F2 m2 = f2(0.f);
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const F2 minus = f2(in[k] ? -mean : 0.f);     // beyond the row: zeros stay zeros
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) {
+                F2& c = v[k * V / 2 + i];
+                c = f2_add(c, minus);
+                m2 = f2_fma(c, c, m2);
+            }
+        }
+        const float var = group_sum(f2_total(m2), p, share + kShare) * per_d;
+        share = (it & 1) ? share - 2 * kShare : share + 2 * kShare;
+        const float rstd = 1.f / sqrtf(var + a.eps);
+        if (live && t == 0) {
+            if (a.mean) a.mean[row] = mean;
+            if (a.rstd) a.rstd[row] = rstd;
+        }
+        const F2 r2 = f2(rstd);
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            F2* h = v + k * V / 2;
+            F2 o[V / 2];
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) {
+                h[i] = f2_mul(h[i], r2);
+                o[i] = f2_fma(h[i], gm[k * V / 2 + i], bt[k * V / 2 + i]);
+            }
+            if (live && in[k]) st_raw<T, V>(dst + k * G * V, pack2<T, V>(o));
+            if constexpr (KEEP != kAsIs) {
+                const uint32_t e = scale_byte(block_amax2<V>(h, live && in[k]), KEEP == kE4M3);
+                if (live && in[k]) {
+                    const int vi = t + k * G;
+                    st_raw<uint8_t, V>(a.q + row * a.d + (int64_t)vi * V, encode2<V>(h, e, KEEP == kE4M3));
+                    if (vi % (kBlock / V) == 0) a.s[row * a.blocks + vi / (kBlock / V)] = (uint8_t)e;
+                }
+            }
+        }
+        dst += a.y_step;
+    }
+}
+
+// dx needs the row again after its sums: g gamma and h stay in registers (HOLD), or the row is read out
+// of the ring a second time and the registers are for the column sums of more columns.
+template <typename T, int E, int STAGES, int THREADS, int KEPT, bool HOLD>
+__global__ void __launch_bounds__(THREADS)
+norm_backward_ring_kernel(NormArgs a) {
+    constexpr int V = 16 / (int)sizeof(T), NV = E / V, SLOT = NV * THREADS;
+    extern __shared__ uint4 ring[];                       // dy: [stage][vector][thread], then x or codes alike
+    __shared__ __align__(16) float2 shares[THREADS / 64][2][kShare];
+    using Code = RawVec<uint8_t, V>;
+    for (int i = threadIdx.x; i < (int)(sizeof(shares) / 8); i += blockDim.x) (&shares[0][0][0])[i] = make_float2(0.f, 0.f);
+    __syncthreads();
+    grid_dependency_wait();
+    const RingPlace p(a.group, a.rows, a.step);
+    const int G = a.group, t = p.t, nvec = (int)(a.d / V), per_block = blockDim.x / G;
+    bool in[NV];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) in[k] = t + k * G < nvec;
+    const T* src = reinterpret_cast<const T*>(a.dy) + p.row * a.lddy + (int64_t)t * V;    // next row to fetch
+    const T* src_x = reinterpret_cast<const T*>(a.x) + p.row * a.ldx + (int64_t)t * V;
+    const uint8_t* src_q = a.q + p.row * a.d + (int64_t)t * V;
+    uint4* own = ring + threadIdx.x;
+    uint4* own_x = ring + STAGES * SLOT + threadIdx.x;
+    Code* own_q = reinterpret_cast<Code*>(ring + STAGES * SLOT) + threadIdx.x;
+    auto fetch = [&](int slot, bool more) {
+        if (more) {
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                if (in[k]) {
+                    ring_copy<16>(own + slot + k * THREADS, src + k * G * V);
+                    if constexpr (KEPT != kAsIs) ring_copy<V>(own_q + slot + k * THREADS, src_q + k * G * V);
+                    else ring_copy<16>(own_x + slot + k * THREADS, src_x + k * G * V);
+                }
+            }
+        }
+        src += a.dy_step;
+        if constexpr (KEPT != kAsIs) src_q += a.q_step; else src_x += a.x_step;
+        cp_async_commit();
+    };
+    // places that no copy fills: the vectors beyond the row read as zeros
+#pragma unroll
+    for (int s = 0; s < STAGES; ++s) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) if (!in[k]) {
+            own[s * SLOT + k * THREADS] = make_uint4(0, 0, 0, 0);
+            if constexpr (KEPT != kAsIs) own_q[s * SLOT + k * THREADS] = Code{};
+            else own_x[s * SLOT + k * THREADS] = make_uint4(0, 0, 0, 0);
+        }
+    }
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; ++s) fetch(s * SLOT, s < p.mine);
+    // gamma lies in shared memory, [vector][quarter][thread of a group]: the registers are taken
+    float4* gammas = reinterpret_cast<float4*>(reinterpret_cast<char*>(ring) + (size_t)STAGES * SLOT * (16 + (KEPT ? V : 16))) + t;
+    if (p.group == 0) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+#pragma unroll
+            for (int j = 0; j < V / 4; ++j) {
+                const int64_t c = (int64_t)(t + k * G) * V + 4 * j;
+                float4 g = make_float4(1.f, 1.f, 1.f, 1.f);
+                if (a.gamma && in[k])
+                    g = make_float4(load_param(a.gamma, a.gamma_f32, dtype_of<T>(), c), load_param(a.gamma, a.gamma_f32, dtype_of<T>(), c + 1),
+                                    load_param(a.gamma, a.gamma_f32, dtype_of<T>(), c + 2), load_param(a.gamma, a.gamma_f32, dtype_of<T>(), c + 3));
+                gammas[(k * (V / 4) + j) * G] = g;
+            }
+        }
+    }
+    __syncthreads();
+    F2 dg[E / 2], db[E / 2];
+#pragma unroll
+    for (int i = 0; i < E / 2; ++i) dg[i] = db[i] = f2(0.f);
+    const float per_d = 1.f / (float)a.d;
+    // what a row needs beside the ring is loaded one row ahead
+    float rstd_next = 0.f, mean_next = 0.f;
+    uint32_t scale[NV] = {};
+    int row = (int)p.row;                                 // fewer than 2^31 rows: a pointer for each of these is two registers
+    auto ahead = [&](int r, bool live) {
+        if (live) {
+            rstd_next = a.rstd[r];
+            if constexpr (KEPT == kAsIs) mean_next = a.mean[r];
+            else {
+                const uint8_t* at = a.s + r * a.blocks + t / (kBlock / V);
+#pragma unroll
+                for (int k = 0; k < NV; ++k) if (in[k]) scale[k] = at[k * G / (kBlock / V)];
+            }
+        }
+    };
+    ahead(row, p.mine > 0);
+    int slot = 0, free_slot = (STAGES - 1) * SLOT;
+    float2* share = &shares[p.warps > 1 ? p.group : 0][0][0];
+    for (int it = 0; it < p.walk; ++it, row += (int)a.step) {
+        const bool live = it < p.mine;
+        const float rstd = rstd_next;
+        const F2 r2 = f2(rstd), minus = f2(-mean_next);
+        cp_async_wait<STAGES - 2>();
+        auto load_dy = [&](int k, F2* g) { unpack2<T, V>(own[slot + k * THREADS], g); };
+        auto load_h = [&](int k, F2* h) {
+            if constexpr (KEPT != kAsIs) {
+                decode2<V>(own_q[slot + k * THREADS], scale[k], KEPT == kE4M3, h);
+            } else {
+                unpack2<T, V>(own_x[slot + k * THREADS], h);
+#pragma unroll
+                for (int i = 0; i < V / 2; ++i) h[i] = f2_mul(f2_add(h[i], minus), r2);
+            }
+        };
+        F2 s1 = f2(0.f), s2 = f2(0.f);
+        F2 gs[HOLD ? E / 2 : V / 2], hs[HOLD ? E / 2 : V / 2];
+        if (live) {                                       // false for groups that share a warp with a longer one
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                F2* g = gs + (HOLD ? k * V / 2 : 0);
+                F2* h = hs + (HOLD ? k * V / 2 : 0);
+                load_dy(k, g);
+                load_h(k, h);
+#pragma unroll
+                for (int q = 0; q < V / 4; ++q) {
+                    const ulonglong2 gm = *reinterpret_cast<const ulonglong2*>(gammas + (k * (V / 4) + q) * G);
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int i = 2 * q + e, j = k * V / 2 + i;
+                        dg[j] = f2_fma(g[i], h[i], dg[j]);
+                        db[j] = f2_add(db[j], g[i]);
+                        g[i] = f2_mul(g[i], e ? gm.y : gm.x);
+                        s1 = f2_add(s1, g[i]);
+                        s2 = f2_fma(g[i], h[i], s2);
+                    }
+                }
+            }
+        }
+        if constexpr (HOLD) {
+            ahead(row + (int)a.step, it + 1 < p.mine);
+            fetch(free_slot, it + STAGES - 1 < p.mine);
+        }
+        const float2 s = group_sum2(f2_total(s1), f2_total(s2), p, share);
+        share = (it & 1) ? share - kShare : share + kShare;
+        if (a.y) {
+            T* dst = reinterpret_cast<T*>(a.y) + row * a.ldy + t * V;
+            const F2 c1 = f2(-s.x * per_d * rstd), c2 = f2(-s.y * per_d * rstd);
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                F2* g = gs + (HOLD ? k * V / 2 : 0);
+                F2* h = hs + (HOLD ? k * V / 2 : 0);
+                if constexpr (!HOLD) load_h(k, h);
+                if constexpr (!HOLD) {
+                    load_dy(k, g);
+#pragma unroll
+                    for (int q = 0; q < V / 4; ++q) {
+                        const ulonglong2 gm = *reinterpret_cast<const ulonglong2*>(gammas + (k * (V / 4) + q) * G);
+                        g[2 * q] = f2_mul(g[2 * q], gm.x);
+                        g[2 * q + 1] = f2_mul(g[2 * q + 1], gm.y);
+                    }
+                }
+                F2 o[V / 2];
+#pragma unroll
+                for (int i = 0; i < V / 2; ++i) o[i] = f2_fma(h[i], c2, f2_fma(g[i], r2, c1));
+                if (live && in[k]) st_raw<T, V>(dst + k * G * V, pack2<T, V>(o));
+            }
+        }
+        if constexpr (!HOLD) {
+            ahead(row + (int)a.step, it + 1 < p.mine);
+            fetch(free_slot, it + STAGES - 1 < p.mine);
+        }
+        free_slot = slot;
+        slot = slot == (STAGES - 1) * SLOT ? 0 : slot + SLOT;
+    }
+    grid_dependency_release();
+    if (!a.partial) return;
+    // Column sums: the groups' side by side in the ring's place, [group][2][d], joined in the groups'
+    // order, so that the order of the sum is fixed.
+    float* column = reinterpret_cast<float*>(ring);
+    const int d2 = 2 * (int)a.d;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        float* c = column + (int64_t)p.group * d2 + (t + k * G) * V;
+        if (in[k]) {
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) {             // in pairs: quads would tie the loop's registers
+                *reinterpret_cast<F2*>(c + 2 * i) = dg[k * V / 2 + i];
+                *reinterpret_cast<F2*>(c + a.d + 2 * i) = db[k * V / 2 + i];
+            }
+        }
+    }
+    __syncthreads();
+    ulonglong2* out = reinterpret_cast<ulonglong2*>(a.partial) + (int64_t)blockIdx.x * (d2 / 4);
+    const ulonglong2* quads = reinterpret_cast<const ulonglong2*>(column);
+#pragma unroll 2
+    for (int q = threadIdx.x; q < d2 / 4; q += blockDim.x) {
+        ulonglong2 sum = quads[q];
+#pragma unroll 4
+        for (int g = 1; g < per_block; ++g) {
+            const ulonglong2 v = quads[g * (d2 / 4) + q];
+            sum.x = f2_add(sum.x, v.x);
+            sum.y = f2_add(sum.y, v.y);
+        }
+        out[q] = sum;
+    }
+}
+
+// Sums the partials: 4 W columns per block (W lanes of four), 1024 / W strands of partials, joined in a
+// fixed order.  VEC: d is a multiple of 4, so four columns are one access.
+template <bool VEC>
+__global__ void __launch_bounds__(1024)
+norm_fold_kernel(const float* partial, int64_t npartials, int64_t d, void* dgamma, void* dbeta, int32_t dtype) {
+    constexpr int W = 16, STRANDS = 1024 / W;
+    __shared__ float part[STRANDS][4 * W + 4];
+    grid_dependency_wait();
+    const int lane = threadIdx.x % W, strand = threadIdx.x / W;
+    const int64_t c = ((int64_t)blockIdx.x * W + lane) * 4;  // over [dgamma | dbeta]
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    // a partial per SM: a strand's three loads are on their way together
+    for (int64_t b = strand; b < npartials; b += STRANDS * 3) {
+        float4 v[3];
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+            v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (b + STRANDS * k >= npartials) continue;
+            const float* at = partial + (b + STRANDS * k) * 2 * d + c;
+            if (VEC) {
+                if (c < 2 * d) v[k] = *reinterpret_cast<const float4*>(at);
+            } else {
+                if (c < 2 * d) v[k].x = at[0];
+                if (c + 1 < 2 * d) v[k].y = at[1];
+                if (c + 2 < 2 * d) v[k].z = at[2];
+                if (c + 3 < 2 * d) v[k].w = at[3];
+            }
+        }
+        sum[0] += v[0].x + v[1].x + v[2].x;
+        sum[1] += v[0].y + v[1].y + v[2].y;
+        sum[2] += v[0].z + v[1].z + v[2].z;
+        sum[3] += v[0].w + v[1].w + v[2].w;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) part[strand][4 * lane + i] = sum[i];
+    __syncthreads();
+    // sixteen threads per column take four strands each
+    const int column = threadIdx.x / 16, fourth = threadIdx.x % 16;
+    float v = (part[fourth][column] + part[fourth + 16][column]) + (part[fourth + 32][column] + part[fourth + 48][column]);
+    v = lane_sum(v, 16);
+    const int64_t cc = (int64_t)blockIdx.x * 4 * W + column;
+    if (fourth != 0 || cc >= 2 * d) return;
+    void* out = cc < d ? dgamma : dbeta;
     if (!out) return;
-    const int64_t i = c < d ? c : c - d;
-    if (dtype == B200_F32) reinterpret_cast<float*>(out)[i] = sum;
-    else if (dtype == B200_F16) reinterpret_cast<__half*>(out)[i] = __float2half_rn(sum);
-    else reinterpret_cast<__nv_bfloat16*>(out)[i] = __float2bfloat16_rn(sum);
+    const int64_t i = cc < d ? cc : cc - d;
+    if (dtype == B200_F32) reinterpret_cast<float*>(out)[i] = v;
+    else if (dtype == B200_F16) reinterpret_cast<__half*>(out)[i] = __float2half_rn(v);
+    else reinterpret_cast<__nv_bfloat16*>(out)[i] = __float2bfloat16_rn(v);
 }
 
 // ---- rows of any length ---------------------------------------------------------------------------
@@ -393,55 +833,99 @@ norm_columns_long_kernel(NormArgs a) {
 }
 
 // ---- host ---------------------------------------------------------------------------------------
-// Threads per row: 16 elements each; at least a whole 8-bit block's lanes.
-static int norm_group(int64_t d, int v) {
+// Threads per row for E elements each: a power of two below a warp (at least a whole 8-bit block's
+// lanes), whole warps above.
+static int ring_group(int64_t d, int e, int v) {
+    const int64_t need = (d + e - 1) / e;
+    if (need > 32) return (int)((need + 31) / 32 * 32);
     int g = v == 1 ? 32 : 8;
+    while (g < need) g *= 2;
+    return g;
+}
+// Threads per row of the element kernels, 16 elements each: a power of two.
+static int norm_group(int64_t d) {
+    int g = 32;
     while ((int64_t)g * kNormElems < d) g *= 2;
     return g;
 }
 static int norm_vector(const NormArgs& a, int32_t dtype, bool aligned) {
     const int v = dtype == B200_F32 ? 4 : 8;
-    return aligned && a.d % v == 0 ? v : 1;
+    return aligned && a.d % v == 0 && a.rows <= 0x3fffffff ? v : 1;    // the ring kernels count rows in 32 bits
+}
+// Dynamic shared memory that with the static one may pass 48 KB has to be allowed once per kernel and device.
+static cudaError_t allow_shared(const void* kernel, size_t bytes, int dev) {
+    if (bytes <= 32 * 1024) return cudaSuccess;
+    static std::mutex mu;
+    static std::vector<std::pair<const void*, int>> done;
+    std::lock_guard<std::mutex> lk(mu);
+    for (const auto& d : done) if (d.first == kernel && d.second == dev) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 219 * 1024);
+    if (e == cudaSuccess) done.emplace_back(kernel, dev);
+    return e;
 }
 
-template <typename T, int V, int NV>
-static cudaError_t launch_forward(b200_stream_t st, const NormArgs& a, int threads) {
-    const int64_t tiles = (a.rows + threads / a.group - 1) / (threads / a.group);
-    auto go = [&](auto kernel) {
-        return launch_overlapped(kernel, balanced_grid(tiles, resident_blocks(kernel, threads, 0, st->dev)), (unsigned)threads, 0, st->s, a);
-    };
-    return a.q ? go(norm_forward_kernel<T, V, NV, true>) : go(norm_forward_kernel<T, V, NV, false>);
+struct NormLaunch {
+    b200_stream_t st;
+    NormArgs a;
+    unsigned threads = 0, grid = 0;
+    size_t smem = 0;
+    // Blocks for a kernel: all resident, each with the same number of rows up to one.
+    template <typename K> cudaError_t plan(K kernel, int per_block, size_t bytes) {
+        threads = (unsigned)(per_block * a.group);
+        smem = bytes;
+        const cudaError_t e = allow_shared(reinterpret_cast<const void*>(kernel), smem, st->dev);
+        if (e != cudaSuccess) return e;
+        grid = balanced_grid((a.rows + per_block - 1) / per_block, resident_blocks(kernel, (int)threads, smem, st->dev));
+        return cudaSuccess;
+    }
+    template <typename K> cudaError_t go(K kernel) {
+        a.step = (int64_t)grid * (threads / a.group);
+        a.x_step = a.step * a.ldx; a.y_step = a.step * a.ldy; a.dy_step = a.step * a.lddy;
+        a.q_step = a.step * a.d;
+        return launch_overlapped(kernel, grid, threads, smem, st->s, a);
+    }
+};
+
+template <typename T, int E, int STAGES, int THREADS>
+static cudaError_t forward_ring(b200_stream_t st, const NormArgs& a) {
+    NormLaunch l{st, a};
+    const int per = a.group >= 256 ? 1 : 256 / a.group;
+    const size_t bytes = (size_t)STAGES * (E * sizeof(T)) * THREADS;
+    auto run = [&](auto kernel) { const cudaError_t e = l.plan(kernel, per, bytes); return e == cudaSuccess ? l.go(kernel) : e; };
+    if (!a.q) return run(norm_forward_ring_kernel<T, E, STAGES, THREADS, kAsIs>);
+    return a.e4m3 ? run(norm_forward_ring_kernel<T, E, STAGES, THREADS, kE4M3>) : run(norm_forward_ring_kernel<T, E, STAGES, THREADS, kInt8>);
 }
 template <typename T>
 static cudaError_t run_forward(b200_stream_t st, NormArgs a, int v) {
-    constexpr int FV = 16 / (int)sizeof(T);
-    a.group = norm_group(a.d, v);
-    if (a.group > kNormMaxGroup)
-        return launch_overlapped(norm_forward_long_kernel<T>, balanced_grid(a.rows, (int64_t)sm_count(st->dev) * 2), 1024u, 0, st->s, a);
-    const int threads = a.group > kNormThreads ? a.group : kNormThreads;
-    return v == 1 ? launch_forward<T, 1, kNormElems>(st, a, threads) : launch_forward<T, FV, kNormElems / FV>(st, a, threads);
+    if (v > 1) {
+        a.group = ring_group(a.d, 32, v);
+        if (a.group <= 256) return forward_ring<T, 32, 3, 256>(st, a);
+        if (a.group <= 512) return forward_ring<T, 32, 3, 512>(st, a);
+    } else {
+        a.group = norm_group(a.d);
+        if (a.group <= kNormMaxGroup) {
+            NormLaunch l{st, a};
+            auto run = [&](auto kernel) { const cudaError_t e = l.plan(kernel, a.group >= kNormThreads ? 1 : kNormThreads / a.group, 0); return e == cudaSuccess ? l.go(kernel) : e; };
+            return a.q ? run(norm_forward_kernel<T, 1, kNormElems, true>) : run(norm_forward_kernel<T, 1, kNormElems, false>);
+        }
+    }
+    return launch_overlapped(norm_forward_long_kernel<T>, balanced_grid(a.rows, (int64_t)sm_count(st->dev) * 2), 1024u, 0, st->s, a);
 }
 
-template <typename T>
-struct NormBackward {
-    static constexpr int FV = 16 / (int)sizeof(T);
-    b200_stream_t st;
-    NormArgs a;
-    int v, threads = 0;
-    unsigned grid = 0;
-    size_t smem = 0;
-
-    template <typename K> void plan(K kernel) {
-        threads = a.group > kNormThreads ? a.group : kNormThreads;
-        const int per = threads / a.group;
-        smem = per > 1 ? 2 * a.d * sizeof(float) : 0;
-        grid = balanced_grid((a.rows + per - 1) / per, resident_blocks(kernel, threads, smem, st->dev));
-    }
-    template <typename F> cudaError_t with_kernel(F f) {
-        if (v == 1) return a.q ? f(norm_backward_kernel<T, 1, kNormElems, true>) : f(norm_backward_kernel<T, 1, kNormElems, false>);
-        return a.q ? f(norm_backward_kernel<T, FV, kNormElems / FV, true>) : f(norm_backward_kernel<T, FV, kNormElems / FV, false>);
-    }
-};
+// Gradient: plans first (the number of blocks sizes the workspace), then launches.
+template <typename T, int E, int STAGES, int THREADS, int KEPT, bool HOLD, typename F>
+static int32_t backward_ring(NormLaunch& l, F space) {
+    constexpr int V = 16 / (int)sizeof(T);
+    const int per = THREADS / l.a.group;
+    size_t bytes = (size_t)STAGES * (E / V) * (16 + (KEPT ? V : 16)) * THREADS + (size_t)E * l.a.group * sizeof(float);
+    const size_t columns = (size_t)per * 2 * l.a.d * sizeof(float);
+    if (bytes < columns) bytes = columns;
+    auto kernel = norm_backward_ring_kernel<T, E, STAGES, THREADS, KEPT, HOLD>;
+    B200_CUDA(l.plan(kernel, per, bytes));
+    B200_TRY(space((int64_t)l.grid));
+    B200_CUDA(l.go(kernel));
+    return B200_OK;
+}
 
 // Workspace of one call.  Outside a capture it is the stream's scratch; inside one the graph gets an
 // allocation of its own, so that graphs captured on one stream can be replayed side by side.
@@ -462,30 +946,61 @@ struct NormSpace {
 
 template <typename T>
 static int32_t run_backward(b200_stream_t st, NormArgs a, int v, void* dgamma, void* dbeta, int32_t ptype) {
+    constexpr bool k16 = sizeof(T) == 2;
     const bool columns = dgamma || dbeta;
     NormSpace space{st};
-    a.group = norm_group(a.d, v);
-    int64_t blocks;
-    if (a.group <= kNormMaxGroup) {
-        NormBackward<T> b{st, a, v};
-        b.with_kernel([&](auto k) { b.plan(k); return cudaSuccess; });
-        blocks = b.grid;
-        if (columns) B200_TRY(space.get((size_t)blocks * 2 * a.d * sizeof(float), &b.a.partial));
-        a.partial = b.a.partial;
-        B200_CUDA(b.with_kernel([&](auto k) { return launch_overlapped(k, b.grid, (unsigned)b.threads, b.smem, st->s, b.a); }));
+    NormLaunch l{st, a};
+    int64_t blocks = 0;
+    // room for the partials of `n` blocks
+    auto room = [&](int64_t n) -> int32_t {
+        blocks = n;
+        return columns ? space.get((size_t)n * 2 * a.d * sizeof(float), &l.a.partial) : B200_OK;
+    };
+    const int g16 = ring_group(a.d, 16, v), g32 = ring_group(a.d, 32, v);
+    // 32 columns per thread where that holds more rows side by side on an SM than 16 do: fewer
+    // instructions per element (16384 x 4096 BFloat16: 69 us, with 16 columns 80; 8192 x 8192: 93 and 84,
+    // one row per SM either way).  Up to 2048 columns the two differ by less than 5 % either way.
+    const bool wide = k16 && v > 1 && g32 <= 384 && (g16 > 512 || (a.d > 2048 && 384 / g32 > 512 / g16));
+    if (wide) {
+        l.a.group = g32;
+        if constexpr (k16) {
+            if (a.q && a.e4m3) B200_TRY((backward_ring<T, 32, 4, 384, kE4M3, true>(l, room)));
+            else if (a.q) B200_TRY((backward_ring<T, 32, 4, 384, kInt8, true>(l, room)));
+            else B200_TRY((backward_ring<T, 32, 3, 384, kAsIs, true>(l, room)));
+        }
+    } else if (v > 1 && g16 <= 512) {
+        l.a.group = g16;
+        if (a.q && a.e4m3) B200_TRY((backward_ring<T, 16, k16 ? 4 : 3, 512, kE4M3, true>(l, room)));
+        else if (a.q) B200_TRY((backward_ring<T, 16, k16 ? 4 : 3, 512, kInt8, true>(l, room)));
+        else B200_TRY((backward_ring<T, 16, k16 ? 4 : 2, 512, kAsIs, true>(l, room)));
+    } else if (v > 1 && k16 && g32 <= 512) {
+        l.a.group = g32;
+        if constexpr (k16) {
+            if (a.q && a.e4m3) B200_TRY((backward_ring<T, 32, 2, 512, kE4M3, false>(l, room)));
+            else if (a.q) B200_TRY((backward_ring<T, 32, 2, 512, kInt8, false>(l, room)));
+            else B200_TRY((backward_ring<T, 32, 2, 512, kAsIs, false>(l, room)));
+        }
+    } else if (v == 1 && norm_group(a.d) <= kNormMaxGroup) {
+        l.a.group = norm_group(a.d);
+        const int per = l.a.group >= kNormThreads ? 1 : kNormThreads / l.a.group;
+        auto run = [&](auto kernel) -> int32_t {
+            B200_CUDA(l.plan(kernel, per, per > 1 ? 2 * a.d * sizeof(float) : 0));
+            B200_TRY(room(l.grid));
+            B200_CUDA(l.go(kernel));
+            return B200_OK;
+        };
+        B200_TRY(a.q ? run(norm_backward_kernel<T, 1, kNormElems, true>) : run(norm_backward_kernel<T, 1, kNormElems, false>));
     } else {
         const int64_t tiles = (a.d + 31) / 32;
-        blocks = (int64_t)sm_count(st->dev) * 8 / tiles;
-        if (blocks > (a.rows + 7) / 8) blocks = (a.rows + 7) / 8;
-        if (blocks < 1) blocks = 1;
-        if (columns) {
-            B200_TRY(space.get((size_t)blocks * 2 * a.d * sizeof(float), &a.partial));
-            norm_columns_long_kernel<T><<<dim3((unsigned)tiles, (unsigned)blocks), 256, 0, st->s>>>(a);
-        }
-        if (a.y) B200_CUDA(launch_overlapped(norm_backward_long_kernel<T>, balanced_grid(a.rows, (int64_t)sm_count(st->dev) * 2), 1024u, 0, st->s, a));
+        int64_t n = (int64_t)sm_count(st->dev) * 8 / tiles;
+        if (n > (a.rows + 7) / 8) n = (a.rows + 7) / 8;
+        if (n < 1) n = 1;
+        B200_TRY(room(n));
+        if (columns) norm_columns_long_kernel<T><<<dim3((unsigned)tiles, (unsigned)n), 256, 0, st->s>>>(l.a);
+        if (a.y) B200_CUDA(launch_overlapped(norm_backward_long_kernel<T>, balanced_grid(a.rows, (int64_t)sm_count(st->dev) * 2), 1024u, 0, st->s, l.a));
     }
     if (columns) {
-        B200_CUDA(launch_overlapped(norm_fold_kernel, (unsigned)((2 * a.d + 31) / 32), 256u, 0, st->s, (const float*)a.partial, blocks, a.d, dgamma, dbeta, ptype));
+        B200_CUDA(launch_overlapped(a.d % 4 == 0 ? norm_fold_kernel<true> : norm_fold_kernel<false>, (unsigned)((2 * a.d + 63) / 64), 1024u, 0, st->s, (const float*)l.a.partial, blocks, a.d, dgamma, dbeta, ptype));
         B200_TRY(space.release());
     }
     return B200_OK;

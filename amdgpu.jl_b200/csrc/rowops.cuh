@@ -161,6 +161,46 @@ __device__ __forceinline__ RawVec<T, V> pack(const float* v) {
     return r;
 }
 
+// ---- pairs of binary32 ------------------------------------------------------------------------------
+// sm_100 issues one instruction for two neighbouring lanes' worth of binary32 arithmetic; the row
+// kernels are bound by instruction issue once their loads are in flight, so they work in pairs.
+using F2 = unsigned long long;
+__device__ __forceinline__ F2 f2(float lo, float hi) { F2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi)); return r; }
+__device__ __forceinline__ F2 f2(float both) { return f2(both, both); }
+__device__ __forceinline__ float2 f2_parts(F2 v) { float2 r; asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v)); return r; }
+__device__ __forceinline__ float f2_total(F2 v) { const float2 r = f2_parts(v); return r.x + r.y; }
+__device__ __forceinline__ F2 f2_add(F2 a, F2 b) { F2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ F2 f2_mul(F2 a, F2 b) { F2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ F2 f2_fma(F2 a, F2 b, F2 c) { F2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+// Largest magnitude of three, NaN if there is one.
+__device__ __forceinline__ float amax3(float a, float b, float c) { float r; asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c)); return r; }
+
+template <typename T, int V>
+__device__ __forceinline__ void unpack2(const RawVec<T, V>& r, F2* v) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&r);
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+        if constexpr (sizeof(T) == 4) {
+            v[i] = f2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+        } else {
+            const float2 f = Elem<T>::get2(w[i]);
+            v[i] = f2(f.x, f.y);
+        }
+    }
+}
+template <typename T, int V>
+__device__ __forceinline__ RawVec<T, V> pack2(const F2* v) {
+    RawVec<T, V> r;
+    uint32_t* w = reinterpret_cast<uint32_t*>(&r);
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+        const float2 f = f2_parts(v[i]);
+        if constexpr (sizeof(T) == 4) { w[2 * i] = __float_as_uint(f.x); w[2 * i + 1] = __float_as_uint(f.y); }
+        else w[i] = Elem<T>::put2(f.x, f.y);
+    }
+    return r;
+}
+
 // ---- 8-bit codec --------------------------------------------------------------------------------
 // A block of 32 values shares the scale 2^(e-127): the smallest power of two, at least 2^-127, that
 // brings the largest magnitude to 127 (Int8) or 448 (e4m3).  Value over scale is exact, so a code is
@@ -250,6 +290,62 @@ __device__ __forceinline__ void decode(const RawVec<uint8_t, V>& r, uint32_t e, 
                 v[4 * i + 2] = (__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7442)) - 8388736.f) * s;
                 v[4 * i + 3] = (__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7443)) - 8388736.f) * s;
             }
+        }
+    }
+}
+// The same for pairs.
+template <int V>
+__device__ __forceinline__ float block_amax2(const F2* v, bool in) {
+    const float2 a = f2_parts(v[0]);
+    float m = amax3(a.x, a.y, 0.f);
+#pragma unroll
+    for (int i = 1; i < V / 2; ++i) { const float2 b = f2_parts(v[i]); m = amax3(m, b.x, b.y); }
+    if (!in) m = 0.f;
+#pragma unroll
+    for (int o = kBlock / V / 2; o > 0; o /= 2) m = jl_max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    return m;
+}
+template <int V>
+__device__ __forceinline__ RawVec<uint8_t, V> encode2(const F2* v, uint32_t e, bool e4m3) {
+    RawVec<uint8_t, V> r{};
+    if (e == 255u) return r;
+    const F2 inv = f2(inverse_scale(e));
+    uint32_t* w = reinterpret_cast<uint32_t*>(&r);
+    if (e4m3) {
+#pragma unroll
+        for (int i = 0; i < V / 4; ++i) {
+            const float2 a = f2_parts(f2_mul(v[2 * i], inv)), b = f2_parts(f2_mul(v[2 * i + 1], inv));
+            w[i] = e4m3_pair(a.x, a.y) | e4m3_pair(b.x, b.y) << 16;
+        }
+    } else {
+        const F2 magic = f2(12582912.f);
+#pragma unroll
+        for (int i = 0; i < V / 4; ++i) {
+            const float2 a = f2_parts(f2_fma(v[2 * i], inv, magic)), b = f2_parts(f2_fma(v[2 * i + 1], inv, magic));
+            const uint32_t lo = __byte_perm(__float_as_uint(a.x), __float_as_uint(a.y), 0x0040);
+            const uint32_t hi = __byte_perm(__float_as_uint(b.x), __float_as_uint(b.y), 0x0040);
+            w[i] = __byte_perm(lo, hi, 0x5410);
+        }
+    }
+    return r;
+}
+template <int V>
+__device__ __forceinline__ void decode2(const RawVec<uint8_t, V>& r, uint32_t e, bool e4m3, F2* v) {
+    const F2 s = f2(scale_value(e));
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&r);
+#pragma unroll
+    for (int i = 0; i < V / 4; ++i) {
+        if (e4m3) {
+            const float2 a = e4m3_values((uint16_t)(w[i] & 0xffffu)), b = e4m3_values((uint16_t)(w[i] >> 16));
+            v[2 * i] = f2_mul(f2(a.x, a.y), s);
+            v[2 * i + 1] = f2_mul(f2(b.x, b.y), s);
+        } else {
+            const uint32_t u = w[i] ^ 0x80808080u;
+            const F2 zero = f2(-8388736.f);
+            const F2 a = f2(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440)), __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7441)));
+            const F2 b = f2(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7442)), __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7443)));
+            v[2 * i] = f2_mul(f2_add(a, zero), s);
+            v[2 * i + 1] = f2_mul(f2_add(b, zero), s);
         }
     }
 }
