@@ -242,8 +242,6 @@ __device__ __forceinline__ RawVec<uint8_t, V> fetch_codes(const RowsArgs& a, con
 }
 // Four codes.  PLAIN: the block's scale is far from overflowing anything; else values past the type's range
 // saturate, and NaN comes out.
-template <typename T>
-__device__ __forceinline__ bool plain_scale(uint32_t e) { return e <= (sizeof(T) == 2 && Elem<T>::kMax < 1e5f ? 134u : 200u); }
 template <typename T, int F, bool PLAIN>
 __device__ __forceinline__ void decode_quad(uint32_t w, uint32_t e, F2* v) {
     if constexpr (PLAIN) {

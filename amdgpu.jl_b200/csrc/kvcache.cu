@@ -27,6 +27,8 @@ struct CacheArgs {
     int64_t tokens, nslots, npages, pl, pb, most, places, seqs;   // pl, pb: strides of the page table
     int64_t islots, ipos, ilengths;                               // their strides
     int32_t heads, page, rot, half, slots_wide, pos_wide, pages_wide, lengths_wide, e4m3, group;
+    int32_t tile, parts, wide;                                    // reading: tokens of a block, blocks of a token; 32-byte accesses
+    FastDiv per_page, per_token;
     float factor;
 };
 
@@ -43,38 +45,39 @@ cache_claim_kernel(CacheArgs a) {
     if (slot >= 1 && slot <= a.nslots) atomicMax(a.owner + slot - 1, (uint32_t)t + 1u);
 }
 
-// V elements from place i of one head of a token, turned if `rot` reaches there.
+// V elements at `p`: 32 bytes are one access where `wide` says that they are aligned.
 template <typename T, int V>
-__device__ __forceinline__ void load_turned(const T* x, int i, int rot, bool half, const float2* turn, float* v) {
-    unpack<T, V>(ld_raw_cached<T, V>(x + i), v);
-    if (i >= rot) return;
-    if (half) {
-        const int h = rot / 2;
-        const bool low = i < h;
-        float p[V];
-        unpack<T, V>(ld_raw_cached<T, V>(x + (low ? i + h : i - h)), p);
-        const float2* w = turn + (low ? i : i - h);
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = fmaf(v[j], w[j].x, (low ? -p[j] : p[j]) * w[j].y);
-    } else if constexpr (V == 1) {
-        const float p = Elem<T>::get(x[i ^ 1]);
-        const float2 w = turn[i / 2];
-        v[0] = fmaf(v[0], w.x, (i & 1 ? p : -p) * w.y);
-    } else {
-#pragma unroll
-        for (int j = 0; j < V / 2; ++j) {
-            const float2 w = turn[i / 2 + j];
-            const float x0 = v[2 * j], x1 = v[2 * j + 1];
-            v[2 * j] = fmaf(x0, w.x, -(x1 * w.y));
-            v[2 * j + 1] = fmaf(x1, w.x, x0 * w.y);
-        }
-    }
+__device__ __forceinline__ RawVec<T, V> load_row(const T* p, bool wide) {
+    if constexpr (sizeof(T) * V == 32) return ld_raw32(p, wide);
+    else return ld_raw_cached<T, V>(p);
+}
+template <typename T, int V>
+__device__ __forceinline__ void unpack_any(const RawVec<T, V>& r, F2* v) {
+    if constexpr (V == 1) { float x; unpack<T, 1>(r, &x); v[0] = f2(x, 0.f); }
+    else unpack2<T, V>(r, v);
 }
 
-// `group` threads (whole warps) per token; the 32/V lanes of a block of 32 are neighbours.
+// One vector of a token: which side, head and place in it.
+struct CacheUnit { bool key, in; int h, i; };
+template <int V>
+__device__ __forceinline__ CacheUnit cache_unit(const CacheArgs& a, int u) {
+    CacheUnit c;
+    c.key = u < a.k.units;
+    if (!c.key) u -= a.k.units;
+    const CacheSide& side = c.key ? a.k : a.v;
+    const bool some = u < side.units;
+    c.h = some ? (int)side.per_head.div((uint32_t)u) : 0;
+    c.i = some ? (u - c.h * (int)side.per_head.d) * V : 0;
+    c.in = some && c.i < side.d;
+    return c;
+}
+
+// `group` threads (whole warps) per token; the 32/V lanes of a block of 32 are neighbours.  A thread's first
+// vectors are on their way while the slot is looked at and the angles are worked out.
 template <typename T, int V>
 __global__ void __launch_bounds__(256)
 cache_write_kernel(CacheArgs a) {
+    constexpr int P = V == 1 ? 1 : V / 2;
     extern __shared__ float2 turns[];            // [tokens of the block][rot / 2] cosine, sine
     __shared__ int lost[8];
     grid_dependency_wait();
@@ -82,6 +85,20 @@ cache_write_kernel(CacheArgs a) {
     const int64_t t = (int64_t)blockIdx.x * (256 / G) + group;
     const bool live = t < a.tokens;
     float2* turn = turns + group * (a.rot / 2);
+    const int half = a.rot / 2;
+    RawVec<T, V> own{}, other{};
+    auto load = [&](const CacheUnit& c) {
+        if (!c.in || !live) return;
+        const CacheSide& side = c.key ? a.k : a.v;
+        const T* x = reinterpret_cast<const T*>(side.x) + t * side.xt + c.h * side.xh;
+        own = load_row<T, V>(x + c.i, a.wide);
+        if (c.key && c.i < a.rot) {
+            if (a.half) other = load_row<T, V>(x + (c.i < half ? c.i + half : c.i - half), a.wide);
+            else if constexpr (V == 1) other = load_row<T, 1>(x + (c.i ^ 1), false);
+        }
+    };
+    CacheUnit c = cache_unit<V>(a, lane);
+    load(c);
     if (lane == 0) lost[group] = 0;
     __syncthreads();
     const int64_t slot = live ? load_int(a.slots, a.slots_wide, t * a.islots) : 0;
@@ -97,65 +114,145 @@ cache_write_kernel(CacheArgs a) {
         }
         if (a.rot) {
             const uint64_t pos = (uint64_t)load_int(a.pos, a.pos_wide, t * a.ipos);
-            for (int i = lane; i < a.rot / 2; i += G) {
-                float s, c;
-                phase_sincos(pos * a.table[i], a.factor, s, c);
-                turn[i] = make_float2(c, s);
+            for (int i = lane; i < half; i += G) {
+                float s, cs;
+                phase_sincos(pos * a.table[i], a.factor, s, cs);
+                turn[i] = make_float2(cs, s);
             }
         }
     }
     __syncthreads();
     const bool write = ok && !lost[group];
-    const int64_t page = ok ? (slot - 1) / a.page : 0, place = ok ? (slot - 1) - page * a.page : 0;
-    for (int base = 0; base < a.k.units + a.v.units; base += G) {
-        int u = base + lane;
-        const bool key = u < a.k.units;
-        if (!key) u -= a.k.units;
-        const CacheSide& side = key ? a.k : a.v;
-        const bool some = write && u < side.units;
-        const int h = some ? (int)side.per_head.div((uint32_t)u) : 0;
-        const int i = some ? (u - h * (int)side.per_head.d) * V : 0;
-        const bool in = some && i < side.d;
-        float v[V];
+    int64_t page = 0, place = 0;
+    if (ok) {
+        if (a.nslots < (int64_t)1 << 31) page = a.per_page.div((uint32_t)(slot - 1));
+        else page = (slot - 1) / a.page;
+        place = slot - 1 - page * a.page;
+    }
+    for (int base = 0;;) {
+        const CacheSide& side = c.key ? a.k : a.v;
+        F2 v[P], p[P];
+        unpack_any<T, V>(own, v);
+        if (c.in && c.key && c.i < a.rot) {
+            unpack_any<T, V>(other, p);
+            if (a.half) {
+                const bool low = c.i < half;
+                const float2* w = turn + (low ? c.i : c.i - half);
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = 0.f;
-        if (in) load_turned<T, V>(reinterpret_cast<const T*>(side.x) + t * side.xt + h * side.xh, i, key ? a.rot : 0, a.half, turn, v);
-        const uint32_t e = scale_byte(block_amax<V>(v), a.e4m3);
-        if (in) {
-            *reinterpret_cast<RawVec<uint8_t, V>*>(side.q + page * side.qn + place * side.qp + h * side.qh + i) = encode<V>(v, e, a.e4m3);
-            if (i % kBlock == 0) side.s[page * side.sn + place * side.sp + h * side.sh + i / kBlock] = (uint8_t)e;
+                for (int j = 0; j < P; ++j) {
+                    const float2 w0 = w[2 * j], w1 = V == 1 ? w0 : w[2 * j + 1];
+                    v[j] = f2_fma(v[j], f2(w0.x, w1.x), f2_mul(p[j], low ? f2(-w0.y, -w1.y) : f2(w0.y, w1.y)));
+                }
+            } else if constexpr (V == 1) {
+                const float2 w = turn[c.i / 2], x = f2_parts(v[0]), y = f2_parts(p[0]);
+                v[0] = f2(fmaf(x.x, w.x, (c.i & 1 ? y.x : -y.x) * w.y), 0.f);
+            } else {
+#pragma unroll
+                for (int j = 0; j < P; ++j) {
+                    const float2 w = turn[c.i / 2 + j], x = f2_parts(v[j]);
+                    v[j] = f2_fma(v[j], f2(w.x), f2_mul(f2(x.y, x.x), f2(-w.y, w.y)));
+                }
+            }
         }
+        const bool in = c.in && write;
+        uint8_t* q = side.q + page * side.qn + place * side.qp + c.h * side.qh + c.i;
+        uint32_t e;
+        if constexpr (V == 1) {
+            float x = c.in ? f2_parts(v[0]).x : 0.f;
+            e = scale_byte(block_amax<1>(&x), a.e4m3);
+            if (in) *q = encode<1>(&x, e, a.e4m3);
+        } else {
+            e = scale_byte(block_amax2<V>(v, c.in), a.e4m3);
+            if (in) *reinterpret_cast<RawVec<uint8_t, V>*>(q) = encode2<V>(v, e, a.e4m3);
+        }
+        if (in && c.i % kBlock == 0) side.s[page * side.sn + place * side.sp + c.h * side.sh + c.i / kBlock] = (uint8_t)e;
+        base += G;
+        if (base >= a.k.units + a.v.units) break;
+        c = cache_unit<V>(a, base + lane);
+        own = other = RawVec<T, V>{};
+        load(c);
     }
 }
+
+// A block reads kTile vectors of one sequence, a whole number of tokens or a part of one.  A thread looks up
+// its four pages together, then loads its four vectors together.
+constexpr int kReadUnroll = 4;
 
 template <typename T, int V>
 __global__ void __launch_bounds__(256)
 cache_read_kernel(CacheArgs a) {
     grid_dependency_wait();
     const int per_token = a.k.units + a.v.units;
-    const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int64_t l = n / per_token;
+    const int64_t cap = min(a.places, a.most * a.page);
+    const int64_t l0 = (int64_t)(blockIdx.x / a.parts) * a.tile;
+    const int part = (int)(blockIdx.x % a.parts) * (256 * kReadUnroll);       // of a token that one block cannot hold
     for (int64_t b = blockIdx.y; b < a.seqs; b += gridDim.y) {
         int64_t length = load_int(a.lengths, a.lengths_wide, b * a.ilengths);
-        const int64_t cap = min(a.places, a.most * a.page);
         if (length < 0 || length > cap) {
-            if (n == 0) latch_error(a.err, B200_INVALID_ARG);
+            if (blockIdx.x == 0 && threadIdx.x == 0) latch_error(a.err, B200_INVALID_ARG);
             length = length < 0 ? 0 : cap;
         }
-        if (l >= length) continue;
-        const int64_t pi = l / a.page, place = l - pi * a.page;
-        const int64_t page = load_int(a.pages, a.pages_wide, pi * a.pl + b * a.pb) - 1;
-        if (page < 0 || page >= a.npages) { latch_error(a.err, B200_INVALID_ARG); continue; }
-        int u = (int)(n - l * per_token);
-        const bool key = u < a.k.units;
-        if (!key) u -= a.k.units;
-        const CacheSide& side = key ? a.k : a.v;
-        const int h = (int)side.per_head.div((uint32_t)u);
-        const int i = (u - h * (int)side.per_head.d) * V;
-        float v[V];
-        decode_as<T, V>(ld_raw<uint8_t, V>(side.q + page * side.qn + place * side.qp + h * side.qh + i),
-                        side.s[page * side.sn + place * side.sp + h * side.sh + i / kBlock], a.e4m3, v);
-        st_raw<T, V>(reinterpret_cast<T*>(side.out) + b * side.ob + l * side.ol + h * side.oh + i, pack<T, V>(v));
+        if (l0 >= length) continue;
+        const int left = (int)min((int64_t)a.tile, length - l0);              // tokens of this block
+        const CacheSide* side[kReadUnroll];
+        int64_t page[kReadUnroll];
+        int place[kReadUnroll], lt[kReadUnroll], h[kReadUnroll], i[kReadUnroll];
+#pragma unroll
+        for (int k = 0; k < kReadUnroll; ++k) {
+            int u = part + k * 256 + threadIdx.x;
+            lt[k] = (int)a.per_token.div((uint32_t)u);
+            u -= lt[k] * per_token;
+            const bool key = u < a.k.units;
+            if (!key) u -= a.k.units;
+            side[k] = key ? &a.k : &a.v;
+            h[k] = (int)side[k]->per_head.div((uint32_t)u);
+            i[k] = (u - h[k] * (int)side[k]->per_head.d) * V;
+            page[k] = -1;
+            if (lt[k] >= left) continue;
+            const uint32_t l = (uint32_t)(l0 + lt[k]), pi = a.per_page.div(l);
+            place[k] = (int)(l - pi * a.per_page.d);
+            page[k] = load_int(a.pages, a.pages_wide, (int64_t)pi * a.pl + b * a.pb) - 1;
+        }
+        RawVec<uint8_t, V> r[kReadUnroll];
+        uint32_t e[kReadUnroll];
+#pragma unroll
+        for (int k = 0; k < kReadUnroll; ++k) {
+            if (lt[k] >= left) continue;
+            if (page[k] < 0 || page[k] >= a.npages) { latch_error(a.err, B200_INVALID_ARG); page[k] = -1; continue; }
+            const CacheSide& s = *side[k];
+            r[k] = ld_raw<uint8_t, V>(s.q + page[k] * s.qn + place[k] * s.qp + h[k] * s.qh + i[k]);
+            e[k] = s.s[page[k] * s.sn + place[k] * s.sp + h[k] * s.sh + i[k] / kBlock];
+        }
+#pragma unroll
+        for (int k = 0; k < kReadUnroll; ++k) {
+            if (lt[k] >= left || page[k] < 0) continue;
+            const CacheSide& s = *side[k];
+            T* out = reinterpret_cast<T*>(s.out) + b * s.ob + (l0 + lt[k]) * s.ol + h[k] * s.oh + i[k];
+            if constexpr (V == 1) {
+                float v;
+                decode_as<T, 1>(r[k], e[k], a.e4m3, &v);
+                st_raw<T, 1>(out, pack<T, 1>(&v));
+            } else {
+                const uint32_t* w = reinterpret_cast<const uint32_t*>(&r[k]);
+                RawVec<T, V> o;
+                uint32_t* po = reinterpret_cast<uint32_t*>(&o);
+#pragma unroll
+                for (int j = 0; j < V / 4; ++j) {
+                    F2 v[2];
+                    if (plain_scale<T>(e[k])) {
+                        decode2<4>(w[j], e[k], a.e4m3, v);
+                    } else {
+                        float x[4];
+                        decode_as<T, 4>(w[j], e[k], a.e4m3, x);
+                        v[0] = f2(x[0], x[1]);
+                        v[1] = f2(x[2], x[3]);
+                    }
+                    *reinterpret_cast<RawVec<T, 4>*>(po + (int)sizeof(T) * j) = pack2<T, 4>(v);
+                }
+                if constexpr (sizeof(T) * V == 32) st_raw32(out, o, a.wide);
+                else st_raw<T, V>(out, o);
+            }
+        }
     }
 }
 
@@ -216,11 +313,11 @@ static int32_t no_overlap(const b200_tensor* t, const char* name) {
 
 template <typename F>
 static cudaError_t by_row_type(int32_t dtype, int v, F f) {
-    switch (dtype) {
-        case B200_F16: return v == 1 ? f(__half{}, std::integral_constant<int, 1>{}) : f(__half{}, std::integral_constant<int, 8>{});
-        case B200_BF16: return v == 1 ? f(__nv_bfloat16{}, std::integral_constant<int, 1>{}) : f(__nv_bfloat16{}, std::integral_constant<int, 8>{});
-        default: return v == 1 ? f(float{}, std::integral_constant<int, 1>{}) : f(float{}, std::integral_constant<int, 4>{});
-    }
+    auto width = [&](auto t) {
+        constexpr int FV = 32 / (int)sizeof(t);
+        return v == 1 ? f(t, std::integral_constant<int, 1>{}) : v == FV ? f(t, std::integral_constant<int, FV>{}) : f(t, std::integral_constant<int, FV / 2>{});
+    };
+    return dtype == B200_F16 ? width(__half{}) : dtype == B200_BF16 ? width(__nv_bfloat16{}) : width(float{});
 }
 
 }  // namespace b200
@@ -260,10 +357,13 @@ extern "C" int32_t b200_cache_write(b200_stream_t st, const b200_tensor* KQ, con
     a.k.x = K->ptr; a.k.xh = K->stride[1]; a.k.xt = K->stride[2];
     a.v.x = V->ptr; a.v.xh = V->stride[1]; a.v.xt = V->stride[2];
     a.err = device_error_word(st->dev);
-    const int fv = dtype == B200_F32 ? 4 : 8;
-    const bool vec = a.k.d % fv == 0 && a.v.d % fv == 0 && multiple_strides(K, fv, 16) && multiple_strides(V, fv, 16) &&
-                     multiple_strides(KQ, fv, (size_t)fv) && multiple_strides(VQ, fv, (size_t)fv) && (a.half ? a.rot / 2 : a.rot) % fv == 0;
-    const int v = vec ? fv : 1;
+    auto fits = [&](int w) {
+        return a.k.d % w == 0 && a.v.d % w == 0 && multiple_strides(K, w, 16) && multiple_strides(V, w, 16) &&
+               multiple_strides(KQ, w, (size_t)w) && multiple_strides(VQ, w, (size_t)w) && (a.half ? a.rot / 2 : a.rot) % w == 0;
+    };
+    const int full = dtype == B200_F32 ? 8 : 16, v = fits(full) ? full : fits(full / 2) ? full / 2 : 1;
+    a.wide = multiple_strides(K, full, 32) && multiple_strides(V, full, 32) && (!a.half || a.rot / 2 % full == 0);
+    a.per_page = FastDiv((uint32_t)a.page);
     for (CacheSide* s : {&a.k, &a.v}) {
         const int per = (int)(row_blocks(s->d) * (kBlock / v));
         s->units = per * a.heads;
@@ -317,16 +417,24 @@ extern "C" int32_t b200_cache_read(b200_stream_t st, const b200_tensor* K, const
     a.k.out = K->ptr; a.k.oh = K->stride[1]; a.k.ol = K->stride[2]; a.k.ob = K->stride[3];
     a.v.out = V->ptr; a.v.oh = V->stride[1]; a.v.ol = V->stride[2]; a.v.ob = V->stride[3];
     a.err = device_error_word(st->dev);
-    const int fv = dtype == B200_F32 ? 4 : 8;
-    const bool vec = a.k.d % fv == 0 && a.v.d % fv == 0 && multiple_strides(K, fv, 16) && multiple_strides(V, fv, 16) &&
-                     multiple_strides(KQ, fv, (size_t)fv) && multiple_strides(VQ, fv, (size_t)fv);
-    const int v = vec ? fv : 1;
+    auto fits = [&](int w) {
+        return a.k.d % w == 0 && a.v.d % w == 0 && multiple_strides(K, w, 16) && multiple_strides(V, w, 16) &&
+               multiple_strides(KQ, w, (size_t)w) && multiple_strides(VQ, w, (size_t)w);
+    };
+    const int full = dtype == B200_F32 ? 8 : 16, v = fits(full) ? full : fits(full / 2) ? full / 2 : 1;
+    a.wide = multiple_strides(K, full, 32) && multiple_strides(V, full, 32);
+    a.per_page = FastDiv((uint32_t)a.page);
     for (CacheSide* s : {&a.k, &a.v}) {
         s->units = s->d / v * a.heads;
         s->per_head = FastDiv((uint32_t)(s->d / v));
     }
-    const int64_t n = a.places * (a.k.units + a.v.units);
-    const int64_t bx = n > 0 ? (n + 255) / 256 : 1;                 // one block at least looks at the lengths
+    const int per_token = a.k.units + a.v.units, block = 256 * kReadUnroll;
+    a.per_token = FastDiv((uint32_t)per_token);
+    a.tile = per_token < block ? block / per_token : 1;
+    a.parts = (per_token + block - 1) / block;
+    if (a.places > 0x7fffffff - a.tile) return fail(B200_TOO_LARGE, "cache read: at most 2^31 places");
+    int64_t bx = (a.places + a.tile - 1) / a.tile * a.parts;
+    if (bx < 1) bx = 1;                                             // one block at least looks at the lengths
     if (bx > 0x7fffffff) return fail(B200_TOO_LARGE, "cache read: too many places for one call");
     const dim3 grid((unsigned)bx, (unsigned)(a.seqs < 65535 ? a.seqs : 65535));
     cudaLaunchConfig_t cfg{};

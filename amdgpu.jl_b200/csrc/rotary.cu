@@ -17,43 +17,67 @@ struct RotaryArgs {
     const void* pos;
     const uint64_t* table;
     int64_t xh, x1, x2, yh, y1, y2, p1, p2;     // element strides: head, token dimensions
-    int64_t tokens, units;                      // units: threads per token
-    int32_t d, rot, heads, chunk, turn_units, wide, adjoint, small;
-    int64_t t1;
-    FastDiv per_token, first;
+    int64_t tokens, t1;
+    uint32_t turn_blocks;
+    int32_t d, rot, heads, chunk, turn_units, pass_units, wide, adjoint, small;     // units: threads per token
+    FastDiv per_token, per_pass, first;
     float factor;
 };
 
-// A thread owns one unit of every head of its share of a token: V pairs (half layout; V = 1 also
-// interleaved) or V/2 pairs (interleaved) or V elements that pass through.  Its angles are computed
-// once and used for `chunk` heads.
+// A thread owns one unit of `chunk` heads of a token: V pairs (half layout; V = 1 also interleaved) or V/2
+// pairs (interleaved) or V elements that pass through.  Its angles are worked out once (about 25
+// instructions a pair, as much as turning three heads), and the loads of kHeads heads are on their way
+// together.
+constexpr int kHeads = 4;
+
 template <typename T, int V, bool HALF>
 __global__ void __launch_bounds__(256)
 rotary_kernel(RotaryArgs a) {
     grid_dependency_wait();
     constexpr bool PAIRED = HALF || V == 1;       // two separate vectors per unit
     constexpr int P = PAIRED ? V : V / 2;
-    const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (n >= a.tokens * a.units) return;
-    int64_t token;
-    int unit;
-    if (a.small) {
-        token = a.per_token.div((uint32_t)n);
-        unit = (int)((uint32_t)n - (uint32_t)token * a.per_token.d);
-    } else {
-        token = n / a.units;
-        unit = (int)(n - token * a.units);
-    }
+    // what turns and what passes through in blocks of their own: side by side in a warp one would wait for
+    // the other
+    const bool turns = blockIdx.x < a.turn_blocks;
+    const int64_t n = (int64_t)(blockIdx.x - (turns ? 0 : a.turn_blocks)) * 256 + threadIdx.x;
+    const int units = turns ? a.turn_units : a.pass_units;
+    if (n >= a.tokens * units) return;
+    const FastDiv& per_token = turns ? a.per_token : a.per_pass;
+    const int64_t token = a.small ? (int64_t)per_token.div((uint32_t)n) : n / units;
+    const int unit = (int)(n - token * units);
     const int64_t t2 = a.small ? (int64_t)a.first.div((uint32_t)token) : token / a.t1;
     const int64_t t1 = token - t2 * a.t1;
     const T* x = reinterpret_cast<const T*>(a.x) + t1 * a.x1 + t2 * a.x2;
     T* y = reinterpret_cast<T*>(a.y) + t1 * a.y1 + t2 * a.y2;
     const int h0 = blockIdx.y * a.chunk, h1 = min(a.heads, h0 + a.chunk);
-    if (unit >= a.turn_units) {
-        const int i = a.rot + (unit - a.turn_units) * V;
-        for (int h = h0; h < h1; ++h) st_raw<T, V>(y + h * a.yh + i, ld_raw<T, V>(x + h * a.xh + i));
+    if (!turns) {
+        const int i = a.rot + unit * V;
+        for (int h = h0; h < h1; h += kHeads) {
+            RawVec<T, V> r[kHeads];
+#pragma unroll
+            for (int k = 0; k < kHeads; ++k) if (h + k < h1) r[k] = ld_raw<T, V>(x + (h + k) * a.xh + i);
+#pragma unroll
+            for (int k = 0; k < kHeads; ++k) if (h + k < h1) st_raw<T, V>(y + (h + k) * a.yh + i, r[k]);
+        }
         return;
     }
+    // places of the two members of a pair
+    const int i0 = HALF ? unit * V : V == 1 ? 2 * unit : unit * V;
+    const int i1 = HALF ? i0 + a.rot / 2 : i0 + 1;
+    x += i0;
+    y += i0;
+    RawVec<T, V> r0[kHeads], r1[kHeads];
+    auto load = [&](int h) {
+#pragma unroll
+        for (int k = 0; k < kHeads; ++k) {
+            if (h + k < h1) {
+                const T* at = x + (h + k) * a.xh;
+                r0[k] = ld_raw<T, V>(at);
+                if constexpr (PAIRED) r1[k] = ld_raw<T, V>(at + (i1 - i0));
+            }
+        }
+    };
+    load(h0);
     const uint64_t pos = (uint64_t)load_int(a.pos, a.wide, t1 * a.p1 + t2 * a.p2);
     float sn[P], cs[P];
 #pragma unroll
@@ -61,53 +85,134 @@ rotary_kernel(RotaryArgs a) {
         phase_sincos(pos * a.table[unit * P + i], a.factor, sn[i], cs[i]);
         if (a.adjoint) sn[i] = -sn[i];
     }
-    // places of the two members of a pair
-    const int i0 = HALF ? unit * V : V == 1 ? 2 * unit : unit * V;
-    const int i1 = HALF ? i0 + a.rot / 2 : i0 + 1;
-    for (int h = h0; h < h1; ++h) {
-        const T* xs = x + h * a.xh;
-        T* ys = y + h * a.yh;
-        if constexpr (PAIRED) {
-            const RawVec<T, V> r0 = ld_raw<T, V>(xs + i0), r1 = ld_raw<T, V>(xs + i1);
-            float u[V], v[V], o[V], w[V];
-            unpack<T, V>(r0, u);
-            unpack<T, V>(r1, v);
+    for (int h = h0; h < h1; h += kHeads) {
+        if (h > h0) load(h);
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                o[i] = fmaf(u[i], cs[i], -(v[i] * sn[i]));
-                w[i] = fmaf(v[i], cs[i], u[i] * sn[i]);
-            }
-            st_raw<T, V>(ys + i0, pack<T, V>(o));
-            st_raw<T, V>(ys + i1, pack<T, V>(w));
-        } else {
-            float u[V], o[V];
-            unpack<T, V>(ld_raw<T, V>(xs + i0), u);
+        for (int k = 0; k < kHeads; ++k) {
+            if (h + k >= h1) break;
+            T* ys = y + (h + k) * a.yh;
+            if constexpr (V == 1) {
+                float u, v;
+                unpack<T, 1>(r0[k], &u);
+                unpack<T, 1>(r1[k], &v);
+                const float o = fmaf(u, cs[0], -(v * sn[0])), w = fmaf(v, cs[0], u * sn[0]);
+                st_raw<T, 1>(ys, pack<T, 1>(&o));
+                st_raw<T, 1>(ys + (i1 - i0), pack<T, 1>(&w));
+            } else if constexpr (HALF) {
+                F2 u[V / 2], v[V / 2];
+                unpack2<T, V>(r0[k], u);
+                unpack2<T, V>(r1[k], v);
 #pragma unroll
-            for (int i = 0; i < P; ++i) {
-                o[2 * i] = fmaf(u[2 * i], cs[i], -(u[2 * i + 1] * sn[i]));
-                o[2 * i + 1] = fmaf(u[2 * i + 1], cs[i], u[2 * i] * sn[i]);
+                for (int i = 0; i < V / 2; ++i) {
+                    const F2 c = f2(cs[2 * i], cs[2 * i + 1]), s = f2(sn[2 * i], sn[2 * i + 1]), minus = f2(-sn[2 * i], -sn[2 * i + 1]);
+                    const F2 o = f2_fma(u[i], c, f2_mul(v[i], minus));
+                    v[i] = f2_fma(v[i], c, f2_mul(u[i], s));
+                    u[i] = o;
+                }
+                st_raw<T, V>(ys, pack2<T, V>(u));
+                st_raw<T, V>(ys + (i1 - i0), pack2<T, V>(v));
+            } else {
+                F2 u[V / 2];
+                unpack2<T, V>(r0[k], u);
+#pragma unroll
+                for (int i = 0; i < P; ++i) {
+                    const float2 z = f2_parts(u[i]);
+                    u[i] = f2_fma(u[i], f2(cs[i]), f2_mul(f2(z.y, z.x), f2(-sn[i], sn[i])));
+                }
+                st_raw<T, V>(ys, pack2<T, V>(u));
             }
-            st_raw<T, V>(ys + i0, pack<T, V>(o));
         }
     }
 }
 
+// Vectors of a head whose pairs do not lie vector to vector: rot/2 is no multiple of V (half layout), or
+// the head turns in part (interleaved).  A thread reads its vector at once and, in half
+// layout, the partners one by one; destination and source must be apart, since a vector's partners are
+// other threads' vectors.
+template <typename T, int V, bool HALF>
+__global__ void __launch_bounds__(256)
+rotary_uneven_kernel(RotaryArgs a) {
+    grid_dependency_wait();
+    const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (n >= a.tokens * a.turn_units) return;
+    const int64_t token = a.small ? (int64_t)a.per_token.div((uint32_t)n) : n / a.turn_units;
+    const int i0 = (int)(n - token * a.turn_units) * V;
+    const int64_t t2 = a.small ? (int64_t)a.first.div((uint32_t)token) : token / a.t1;
+    const int64_t t1 = token - t2 * a.t1;
+    const T* x = reinterpret_cast<const T*>(a.x) + t1 * a.x1 + t2 * a.x2;
+    T* y = reinterpret_cast<T*>(a.y) + t1 * a.y1 + t2 * a.y2;
+    const int h0 = blockIdx.y * a.chunk, h1 = min(a.heads, h0 + a.chunk), half = a.rot / 2;
+    float sn[V], cs[V];
+    if (i0 < a.rot) {
+        const uint64_t pos = (uint64_t)load_int(a.pos, a.wide, t1 * a.p1 + t2 * a.p2);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int i = i0 + j;
+            sn[j] = cs[j] = 0.f;
+            if (i >= a.rot || (!HALF && (j & 1))) continue;
+            phase_sincos(pos * a.table[HALF ? (i < half ? i : i - half) : i / 2], a.factor, sn[j], cs[j]);
+            if (a.adjoint) sn[j] = -sn[j];
+            if (HALF && i < half) sn[j] = -sn[j];
+        }
+    }
+    for (int h = h0; h < h1; h += 2) {
+        RawVec<T, V> r[2];
+        float p[2][V];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            if (h + k >= h1) continue;
+            const T* at = x + (h + k) * a.xh;
+            r[k] = ld_raw_cached<T, V>(at + i0);
+            if constexpr (HALF) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const int i = i0 + j;
+                    p[k][j] = i < a.rot ? Elem<T>::get(at[i < half ? i + half : i - half]) : 0.f;
+                }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            if (h + k >= h1) continue;
+            float u[V];
+            unpack<T, V>(r[k], u);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                if constexpr (HALF) {
+                    if (i0 + j < a.rot) u[j] = fmaf(u[j], cs[j], p[k][j] * sn[j]);
+                } else if (!(j & 1) && i0 + j < a.rot) {
+                    const float v = u[j + 1];
+                    u[j + 1] = fmaf(v, cs[j], u[j] * sn[j]);
+                    u[j] = fmaf(u[j], cs[j], -(v * sn[j]));
+                }
+            }
+            st_raw<T, V>(y + (h + k) * a.yh + i0, pack<T, V>(u));
+        }
+    }
+}
+
+enum { kByElement = 0, kVectors = 1, kUneven = 2 };
+
 template <typename T>
-static cudaError_t run_rotary(b200_stream_t st, RotaryArgs a, bool half, bool vec, bool in_place) {
+static cudaError_t run_rotary(b200_stream_t st, RotaryArgs a, bool half, int how, bool in_place) {
     constexpr int FV = 16 / (int)sizeof(T);
-    const int v = vec ? FV : 1;
-    a.turn_units = half || v == 1 ? a.rot / 2 / v : a.rot / v;
-    a.units = a.turn_units + (in_place ? 0 : (a.d - a.rot) / v);
-    const int64_t n = a.tokens * a.units;
+    const int v = how == kByElement ? 1 : FV;
+    a.turn_units = how == kUneven ? a.d / v : half || v == 1 ? a.rot / 2 / v : a.rot / v;
+    a.pass_units = how == kUneven || in_place ? 0 : (a.d - a.rot) / v;
+    const int64_t n = a.tokens * (a.turn_units + a.pass_units);
     a.small = n < (int64_t)1 << 30;
-    a.per_token = FastDiv((uint32_t)a.units);
+    a.per_token = FastDiv((uint32_t)a.turn_units);
+    a.per_pass = FastDiv((uint32_t)a.pass_units);
     a.first = FastDiv((uint32_t)(a.t1 < (int64_t)1 << 30 ? a.t1 : 1));
-    // heads per thread: as many as leave the device four waves of threads
+    // heads per thread: as many as leave every SM two blocks of threads (16384 tokens of 32 + 8 heads of 128:
+    // 58 us; with four or sixteen times the threads, so fewer heads for one set of angles, 62 and 75 us)
     a.chunk = a.heads;
-    while (a.chunk > 1 && n * ((a.heads + a.chunk - 1) / a.chunk) < (int64_t)sm_count(st->dev) * 2048 * 4) a.chunk = (a.chunk + 1) / 2;
+    while (a.chunk > 1 && n * ((a.heads + a.chunk - 1) / a.chunk) < (int64_t)sm_count(st->dev) * 512) a.chunk = (a.chunk + 1) / 2;
     while ((a.heads + a.chunk - 1) / a.chunk > 65535) ++a.chunk;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)((n + 255) / 256), (unsigned)((a.heads + a.chunk - 1) / a.chunk));
+    a.turn_blocks = (uint32_t)((a.tokens * a.turn_units + 255) / 256);
+    const uint32_t pass_blocks = (uint32_t)((a.tokens * a.pass_units + 255) / 256);
+    cfg.gridDim = dim3(a.turn_blocks + pass_blocks, (unsigned)((a.heads + a.chunk - 1) / a.chunk));
     cfg.blockDim = dim3(256);
     cfg.stream = st->s;
     cudaLaunchAttribute attr[1];
@@ -115,6 +220,7 @@ static cudaError_t run_rotary(b200_stream_t st, RotaryArgs a, bool half, bool ve
     attr[0].val.programmaticStreamSerializationAllowed = overlap_launches_enabled() ? 1 : 0;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
+    if (how == kUneven) return half ? cudaLaunchKernelEx(&cfg, rotary_uneven_kernel<T, FV, true>, a) : cudaLaunchKernelEx(&cfg, rotary_uneven_kernel<T, FV, false>, a);
     if (half) return v == 1 ? cudaLaunchKernelEx(&cfg, rotary_kernel<T, 1, true>, a) : cudaLaunchKernelEx(&cfg, rotary_kernel<T, FV, true>, a);
     return v == 1 ? cudaLaunchKernelEx(&cfg, rotary_kernel<T, 1, false>, a) : cudaLaunchKernelEx(&cfg, rotary_kernel<T, FV, false>, a);
 }
@@ -162,15 +268,18 @@ extern "C" int32_t b200_rotary(b200_stream_t st, const b200_tensor* Y, const b20
         return reinterpret_cast<uintptr_t>(t->ptr) % 16 == 0;
     };
     const bool half = layout == kRotaryHalf;
-    const bool vec = strides_ok(X) && strides_ok(Y) && d % fv == 0 && (half ? rot / 2 : rot) % fv == 0;
+    const bool vec = strides_ok(X) && strides_ok(Y) && d % fv == 0;
     bool in_place = X->ptr == Y->ptr;
     for (int k = 1; k < X->ndim; ++k) in_place = in_place && (X->shape[k] == 1 || X->stride[k] == Y->stride[k]);
     if (in_place && rot == 0) return B200_OK;
-    if (a.tokens * (d / (vec ? fv : 1)) / 256 > 0x7ffffff0) return fail(B200_TOO_LARGE, "rotary: too many tokens for one call");
+    // interleaved heads that turn in part go by whole vectors too: one kind of thread for all (16384 tokens of
+    // 16 heads of 96 with 64 turned: 15 us, 18 with blocks apart, 24 with both kinds in a warp)
+    const int how = !vec ? kByElement : half ? (rot / 2 % fv == 0 ? kVectors : in_place ? kByElement : kUneven) : rot == d ? kVectors : kUneven;
+    if (a.tokens * (d / (how == kByElement ? 1 : fv)) / 256 > 0x7ffffff0) return fail(B200_TOO_LARGE, "rotary: too many tokens for one call");
     switch (X->dtype) {
-        case B200_F16: B200_CUDA(run_rotary<__half>(st, a, half, vec, in_place)); break;
-        case B200_BF16: B200_CUDA(run_rotary<__nv_bfloat16>(st, a, half, vec, in_place)); break;
-        default: B200_CUDA(run_rotary<float>(st, a, half, vec, in_place)); break;
+        case B200_F16: B200_CUDA(run_rotary<__half>(st, a, half, how, in_place)); break;
+        case B200_BF16: B200_CUDA(run_rotary<__nv_bfloat16>(st, a, half, how, in_place)); break;
+        default: B200_CUDA(run_rotary<float>(st, a, half, how, in_place)); break;
     }
     return finish(st, "b200_rotary");
 }

@@ -382,6 +382,9 @@ template <typename T>
 __device__ __forceinline__ uint32_t saturating_from(bool e4m3) {
     return sizeof(T) == 2 && Elem<T>::kMax < 1e5f ? (e4m3 ? 135u : 137u) : (e4m3 ? 247u : 249u);
 }
+// Scales that are far from overflowing anything.
+template <typename T>
+__device__ __forceinline__ bool plain_scale(uint32_t e) { return e <= (sizeof(T) == 2 && Elem<T>::kMax < 1e5f ? 134u : 200u); }
 template <typename T, int V>
 __device__ __forceinline__ void decode_as(const RawVec<uint8_t, V>& r, uint32_t e, bool e4m3, float* v) {
     decode<V>(r, e, e4m3, v);
