@@ -9,7 +9,7 @@
 namespace b200 {
 
 enum { kSilu = 0, kGelu = 1 };
-enum { kNoCodes = 0, kInt8 = 1, kE4M3 = 2 };
+enum { kNoCodes = 0 };
 
 // f(a) and f'(a) for binary32 results.  With e = exp(-|u|) and r = 1/(1+e) the sigmoid is r or e r and its
 // derivative e r^2: no cancellation, and nothing overflows.  Beyond 128 the sigmoid is 0 or 1 in binary32
@@ -405,7 +405,7 @@ struct RowsCall {
         *s = (uint8_t*)S->ptr;
         return B200_OK;
     }
-    int format() const { return a.qa || a.qb ? (a.e4m3 ? kE4M3 : kInt8) : kNoCodes; }
+    int format() const { return !(a.qa || a.qb) ? (int)kNoCodes : a.e4m3 ? (int)kE4M3 : (int)kInt8; }
     // Vector width, and the slots for it; 0: nothing to do.
     int plan() {
         if (a.rows == 0 || a.d == 0) return 0;

@@ -27,7 +27,7 @@ struct CacheArgs {
     int64_t tokens, nslots, npages, pl, pb, most, places, seqs;   // pl, pb: strides of the page table
     int64_t islots, ipos, ilengths;                               // their strides
     int32_t heads, page, rot, half, slots_wide, pos_wide, pages_wide, lengths_wide, e4m3, group;
-    int32_t tile, parts, wide;                                    // reading: tokens of a block, blocks of a token; 32-byte accesses
+    int32_t tile, parts, abreast, wide;                           // reading: tokens of a block, blocks of a token, tokens side by side
     FastDiv per_page, per_token;
     float factor;
 };
@@ -72,17 +72,30 @@ __device__ __forceinline__ CacheUnit cache_unit(const CacheArgs& a, int u) {
     return c;
 }
 
+// How keys turn on the way: vector against vector (half layout), within a vector (interleaved), or, where
+// pairs do not lie so, element by element against partners that are read one by one.
+enum { kNoTurn = 0, kTurnHalf = 1, kTurnInterleaved = 2, kTurnUneven = 3 };
+
+// Place of pair i's cosine and sine: the pairs of a thread's vector lie apart, those of neighbouring threads
+// side by side (no bank is asked for twice).
+template <int V, int TURN>
+__device__ __forceinline__ int turn_at(int i, int half) {
+    constexpr int PER = V == 1 || TURN == kTurnUneven ? 1 : TURN == kTurnHalf ? V : V / 2;
+    return PER == 1 ? i : (i % PER) * (half / PER) + i / PER;
+}
+
 // `group` threads (whole warps) per token; the 32/V lanes of a block of 32 are neighbours.  A thread's first
 // vectors are on their way while the slot is looked at and the angles are worked out.
-template <typename T, int V>
-__global__ void __launch_bounds__(256)
+template <typename T, int V, int F, int TURN>
+__global__ void __launch_bounds__(256, TURN == kTurnHalf ? 5 : 1)
 cache_write_kernel(CacheArgs a) {
     constexpr int P = V == 1 ? 1 : V / 2;
     extern __shared__ float2 turns[];            // [tokens of the block][rot / 2] cosine, sine
     __shared__ int lost[8];
+    __shared__ int2 where[8];                    // page and place of a token's slot; page -1: nowhere
     grid_dependency_wait();
     const int G = a.group, group = threadIdx.x / G, lane = threadIdx.x % G;
-    const int64_t t = (int64_t)blockIdx.x * (256 / G) + group;
+    const uint32_t t = blockIdx.x * (256 / G) + group;
     const bool live = t < a.tokens;
     float2* turn = turns + group * (a.rot / 2);
     const int half = a.rot / 2;
@@ -90,57 +103,83 @@ cache_write_kernel(CacheArgs a) {
     auto load = [&](const CacheUnit& c) {
         if (!c.in || !live) return;
         const CacheSide& side = c.key ? a.k : a.v;
-        const T* x = reinterpret_cast<const T*>(side.x) + t * side.xt + c.h * side.xh;
-        own = load_row<T, V>(x + c.i, a.wide);
-        if (c.key && c.i < a.rot) {
-            if (a.half) other = load_row<T, V>(x + (c.i < half ? c.i + half : c.i - half), a.wide);
-            else if constexpr (V == 1) other = load_row<T, 1>(x + (c.i ^ 1), false);
+        const T* x = reinterpret_cast<const T*>(side.x) + (int64_t)t * side.xt + c.h * side.xh + c.i;
+        own = load_row<T, V>(x, a.wide);
+        if (TURN != kNoTurn && c.key && c.i < a.rot) {
+            if constexpr (TURN == kTurnHalf) other = load_row<T, V>(x + (c.i < half ? half : -half), a.wide);
+            else if constexpr (V == 1) other = load_row<T, 1>(x + (c.i & 1 ? -1 : 1), false);
+            else if constexpr (TURN == kTurnUneven) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const int i = c.i + j;
+                    if (i < a.rot) reinterpret_cast<T*>(&other)[j] = x[j + (a.half ? (i < half ? half : -half) : i & 1 ? -1 : 1)];
+                }
+            }
         }
     };
     CacheUnit c = cache_unit<V>(a, lane);
     load(c);
-    if (lane == 0) lost[group] = 0;
+    if (lane == 0) {
+        int2 w = make_int2(-1, 0);
+        lost[group] = 0;
+        if (live) {
+            const int64_t slot = load_int(a.slots, a.slots_wide, t * a.islots);
+            if (slot >= 1 && slot <= a.nslots) {
+                const int64_t page = a.nslots < (int64_t)1 << 31 ? (int64_t)a.per_page.div((uint32_t)(slot - 1)) : (slot - 1) / a.page;
+                w = make_int2((int)page, (int)(slot - 1 - page * a.page));
+                if (a.owner && a.owner[slot - 1] != t + 1u) w.x = -1;
+            } else if (slot != 0) {
+                latch_error(a.err, B200_INVALID_ARG);
+            }
+        }
+        where[group] = w;
+    }
     __syncthreads();
-    const int64_t slot = live ? load_int(a.slots, a.slots_wide, t * a.islots) : 0;
-    const bool ok = slot >= 1 && slot <= a.nslots;
-    if (live && !ok && slot != 0 && lane == 0) latch_error(a.err, B200_INVALID_ARG);
-    if (ok) {
+    const int2 w = where[group];
+    if (w.x >= 0) {
         // of several tokens with one slot the last is kept, as if they were written in turn
-        if (a.owner) {
-            if (lane == 0 && a.owner[slot - 1] != (uint32_t)t + 1u) lost[group] = 1;
-        } else {
+        if (!a.owner && t + 1 < a.tokens) {
+            const int64_t slot = load_int(a.slots, a.slots_wide, t * a.islots);
             for (int64_t j = t + 1 + lane; j < a.tokens; j += G)
                 if (load_int(a.slots, a.slots_wide, j * a.islots) == slot) lost[group] = 1;
         }
-        if (a.rot) {
+        if constexpr (TURN != kNoTurn) {
             const uint64_t pos = (uint64_t)load_int(a.pos, a.pos_wide, t * a.ipos);
             for (int i = lane; i < half; i += G) {
                 float s, cs;
                 phase_sincos(pos * a.table[i], a.factor, s, cs);
-                turn[i] = make_float2(cs, s);
+                turn[turn_at<V, TURN>(i, half)] = make_float2(cs, s);
             }
         }
     }
     __syncthreads();
-    const bool write = ok && !lost[group];
-    int64_t page = 0, place = 0;
-    if (ok) {
-        if (a.nslots < (int64_t)1 << 31) page = a.per_page.div((uint32_t)(slot - 1));
-        else page = (slot - 1) / a.page;
-        place = slot - 1 - page * a.page;
-    }
+    const bool write = w.x >= 0 && !lost[group];
     for (int base = 0;;) {
         const CacheSide& side = c.key ? a.k : a.v;
         F2 v[P], p[P];
         unpack_any<T, V>(own, v);
-        if (c.in && c.key && c.i < a.rot) {
+        if (TURN != kNoTurn && c.in && c.key && c.i < a.rot) {
             unpack_any<T, V>(other, p);
-            if (a.half) {
+            if constexpr (TURN == kTurnUneven) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const int i = c.i + j;
+                    if (i >= a.rot) continue;
+                    const bool first = a.half ? i < half : !(i & 1);
+                    const float2 w = turn[a.half ? (first ? i : i - half) : i / 2];
+                    float2 x = f2_parts(v[j / 2]);
+                    const float2 y = f2_parts(p[j / 2]);
+                    float& z = j & 1 ? x.y : x.x;
+                    z = fmaf(z, w.x, (j & 1 ? y.y : y.x) * (first ? -w.y : w.y));
+                    v[j / 2] = f2(x.x, x.y);
+                }
+            } else if constexpr (TURN == kTurnHalf) {
                 const bool low = c.i < half;
-                const float2* w = turn + (low ? c.i : c.i - half);
+                const float2* w = turn + (low ? c.i : c.i - half) / V;
+                const int step = half / V;
 #pragma unroll
                 for (int j = 0; j < P; ++j) {
-                    const float2 w0 = w[2 * j], w1 = V == 1 ? w0 : w[2 * j + 1];
+                    const float2 w0 = w[2 * j * step], w1 = V == 1 ? w0 : w[(2 * j + 1) * step];
                     v[j] = f2_fma(v[j], f2(w0.x, w1.x), f2_mul(p[j], low ? f2(-w0.y, -w1.y) : f2(w0.y, w1.y)));
                 }
             } else if constexpr (V == 1) {
@@ -149,23 +188,24 @@ cache_write_kernel(CacheArgs a) {
             } else {
 #pragma unroll
                 for (int j = 0; j < P; ++j) {
-                    const float2 w = turn[c.i / 2 + j], x = f2_parts(v[j]);
+                    const float2 w = turn[c.i / V + j * (half / P)], x = f2_parts(v[j]);
                     v[j] = f2_fma(v[j], f2(w.x), f2_mul(f2(x.y, x.x), f2(-w.y, w.y)));
                 }
             }
         }
         const bool in = c.in && write;
-        uint8_t* q = side.q + page * side.qn + place * side.qp + c.h * side.qh + c.i;
+        uint8_t* q = side.q + (int64_t)w.x * (int32_t)side.qn + (int64_t)w.y * (int32_t)side.qp + c.h * side.qh + c.i;
         uint32_t e;
         if constexpr (V == 1) {
             float x = c.in ? f2_parts(v[0]).x : 0.f;
-            e = scale_byte(block_amax<1>(&x), a.e4m3);
-            if (in) *q = encode<1>(&x, e, a.e4m3);
+            e = scale_byte(block_amax<1>(&x), F == kE4M3);
+            if (in) *q = encode<1>(&x, e, F == kE4M3);
         } else {
-            e = scale_byte(block_amax2<V>(v, c.in), a.e4m3);
-            if (in) *reinterpret_cast<RawVec<uint8_t, V>*>(q) = encode2<V>(v, e, a.e4m3);
+            e = scale_byte(block_amax2<V>(v, c.in), F == kE4M3);
+            if (in) *reinterpret_cast<RawVec<uint8_t, V>*>(q) = encode2<V>(v, e, F == kE4M3);
         }
-        if (in && c.i % kBlock == 0) side.s[page * side.sn + place * side.sp + c.h * side.sh + c.i / kBlock] = (uint8_t)e;
+        if (in && c.i % kBlock == 0)
+            side.s[(int64_t)w.x * (int32_t)side.sn + (int64_t)w.y * (int32_t)side.sp + c.h * side.sh + c.i / kBlock] = (uint8_t)e;
         base += G;
         if (base >= a.k.units + a.v.units) break;
         c = cache_unit<V>(a, base + lane);
@@ -174,83 +214,89 @@ cache_write_kernel(CacheArgs a) {
     }
 }
 
-// A block reads kTile vectors of one sequence, a whole number of tokens or a part of one.  A thread looks up
-// its four pages together, then loads its four vectors together.
+// A thread keeps its vector of a token - side, head and place are worked out once - and walks over the
+// tokens of the block's tile, kReadUnroll at a time: their pages are looked up together, then their codes
+// are loaded together.
 constexpr int kReadUnroll = 4;
 
-template <typename T, int V>
+template <typename T, int V, int F>
 __global__ void __launch_bounds__(256)
 cache_read_kernel(CacheArgs a) {
     grid_dependency_wait();
     const int per_token = a.k.units + a.v.units;
     const int64_t cap = min(a.places, a.most * a.page);
-    const int64_t l0 = (int64_t)(blockIdx.x / a.parts) * a.tile;
-    const int part = (int)(blockIdx.x % a.parts) * (256 * kReadUnroll);       // of a token that one block cannot hold
+    const int tile = (int)(blockIdx.x / a.parts), abreast = a.abreast;
+    int u = (int)(blockIdx.x % a.parts) * 256 + threadIdx.x, t0 = 0;      // parts: of a token with more than 256 vectors
+    if (a.parts == 1) { t0 = (int)a.per_token.div((uint32_t)u); u -= t0 * per_token; }
+    const bool idle = u >= per_token;
+    const bool key = u < a.k.units;
+    if (!key) u -= a.k.units;
+    const CacheSide& side = key ? a.k : a.v;
+    const int h = idle ? 0 : (int)side.per_head.div((uint32_t)u);
+    const int i = idle ? 0 : (u - h * (int)side.per_head.d) * V;
+    const uint8_t *q = side.q + h * side.qh + i, *sc = side.s + h * side.sh + i / kBlock;
+    const int32_t qn = (int32_t)side.qn, qp = (int32_t)side.qp, sn = (int32_t)side.sn, sp = (int32_t)side.sp, ol = (int32_t)side.ol;
     for (int64_t b = blockIdx.y; b < a.seqs; b += gridDim.y) {
         int64_t length = load_int(a.lengths, a.lengths_wide, b * a.ilengths);
         if (length < 0 || length > cap) {
             if (blockIdx.x == 0 && threadIdx.x == 0) latch_error(a.err, B200_INVALID_ARG);
             length = length < 0 ? 0 : cap;
         }
-        if (l0 >= length) continue;
-        const int left = (int)min((int64_t)a.tile, length - l0);              // tokens of this block
-        const CacheSide* side[kReadUnroll];
-        int64_t page[kReadUnroll];
-        int place[kReadUnroll], lt[kReadUnroll], h[kReadUnroll], i[kReadUnroll];
+        const int first = tile * a.tile, last = (int)min((int64_t)first + a.tile, length);
+        if (idle) continue;
+        T* out = reinterpret_cast<T*>(side.out) + b * side.ob + h * side.oh + i;
+        for (int l = first + t0; l < last; l += abreast * kReadUnroll) {
+            int64_t page[kReadUnroll];
+            int place[kReadUnroll];
 #pragma unroll
-        for (int k = 0; k < kReadUnroll; ++k) {
-            int u = part + k * 256 + threadIdx.x;
-            lt[k] = (int)a.per_token.div((uint32_t)u);
-            u -= lt[k] * per_token;
-            const bool key = u < a.k.units;
-            if (!key) u -= a.k.units;
-            side[k] = key ? &a.k : &a.v;
-            h[k] = (int)side[k]->per_head.div((uint32_t)u);
-            i[k] = (u - h[k] * (int)side[k]->per_head.d) * V;
-            page[k] = -1;
-            if (lt[k] >= left) continue;
-            const uint32_t l = (uint32_t)(l0 + lt[k]), pi = a.per_page.div(l);
-            place[k] = (int)(l - pi * a.per_page.d);
-            page[k] = load_int(a.pages, a.pages_wide, (int64_t)pi * a.pl + b * a.pb) - 1;
-        }
-        RawVec<uint8_t, V> r[kReadUnroll];
-        uint32_t e[kReadUnroll];
+            for (int k = 0; k < kReadUnroll; ++k) {
+                const int lk = l + k * abreast;
+                page[k] = -1;
+                if (lk >= last) continue;
+                const uint32_t pi = a.per_page.div((uint32_t)lk);
+                place[k] = (int)((uint32_t)lk - pi * a.per_page.d);
+                page[k] = load_int(a.pages, a.pages_wide, (int64_t)pi * a.pl + b * a.pb) - 1;
+                if (page[k] < 0 || page[k] >= a.npages) { latch_error(a.err, B200_INVALID_ARG); page[k] = -1; }
+            }
+            RawVec<uint8_t, V> r[kReadUnroll];
+            uint32_t e[kReadUnroll];
 #pragma unroll
-        for (int k = 0; k < kReadUnroll; ++k) {
-            if (lt[k] >= left) continue;
-            if (page[k] < 0 || page[k] >= a.npages) { latch_error(a.err, B200_INVALID_ARG); page[k] = -1; continue; }
-            const CacheSide& s = *side[k];
-            r[k] = ld_raw<uint8_t, V>(s.q + page[k] * s.qn + place[k] * s.qp + h[k] * s.qh + i[k]);
-            e[k] = s.s[page[k] * s.sn + place[k] * s.sp + h[k] * s.sh + i[k] / kBlock];
-        }
+            for (int k = 0; k < kReadUnroll; ++k) {
+                if (page[k] < 0) continue;
+                const int32_t pg = (int32_t)page[k];
+                e[k] = sc[(int64_t)pg * sn + (int64_t)place[k] * sp];
+                r[k] = ld_raw<uint8_t, V>(q + (int64_t)pg * qn + (int64_t)place[k] * qp);
+            }
 #pragma unroll
-        for (int k = 0; k < kReadUnroll; ++k) {
-            if (lt[k] >= left || page[k] < 0) continue;
-            const CacheSide& s = *side[k];
-            T* out = reinterpret_cast<T*>(s.out) + b * s.ob + (l0 + lt[k]) * s.ol + h[k] * s.oh + i[k];
-            if constexpr (V == 1) {
-                float v;
-                decode_as<T, 1>(r[k], e[k], a.e4m3, &v);
-                st_raw<T, 1>(out, pack<T, 1>(&v));
-            } else {
-                const uint32_t* w = reinterpret_cast<const uint32_t*>(&r[k]);
-                RawVec<T, V> o;
-                uint32_t* po = reinterpret_cast<uint32_t*>(&o);
-#pragma unroll
-                for (int j = 0; j < V / 4; ++j) {
-                    F2 v[2];
+            for (int k = 0; k < kReadUnroll; ++k) {
+                if (page[k] < 0) continue;
+                T* to = out + (int64_t)(l + k * abreast) * ol;
+                if constexpr (V == 1) {
+                    float v;
+                    decode_as<T, 1>(r[k], e[k], F == kE4M3, &v);
+                    st_raw<T, 1>(to, pack<T, 1>(&v));
+                } else {
+                    const uint32_t* w = reinterpret_cast<const uint32_t*>(&r[k]);
+                    RawVec<T, V> o;
+                    uint32_t* po = reinterpret_cast<uint32_t*>(&o);
                     if (plain_scale<T>(e[k])) {
-                        decode2<4>(w[j], e[k], a.e4m3, v);
+#pragma unroll
+                        for (int j = 0; j < V / 4; ++j) {
+                            F2 v[2];
+                            decode2<4>(w[j], e[k], F == kE4M3, v);
+                            *reinterpret_cast<RawVec<T, 4>*>(po + (int)sizeof(T) * j) = pack2<T, 4>(v);
+                        }
                     } else {
-                        float x[4];
-                        decode_as<T, 4>(w[j], e[k], a.e4m3, x);
-                        v[0] = f2(x[0], x[1]);
-                        v[1] = f2(x[2], x[3]);
+#pragma unroll
+                        for (int j = 0; j < V / 4; ++j) {
+                            float x[4];
+                            decode_as<T, 4>(w[j], e[k], F == kE4M3, x);
+                            *reinterpret_cast<RawVec<T, 4>*>(po + (int)sizeof(T) * j) = pack<T, 4>(x);
+                        }
                     }
-                    *reinterpret_cast<RawVec<T, 4>*>(po + (int)sizeof(T) * j) = pack2<T, 4>(v);
+                    if constexpr (sizeof(T) * V == 32) st_raw32(to, o, a.wide);
+                    else st_raw<T, V>(to, o);
                 }
-                if constexpr (sizeof(T) * V == 32) st_raw32(out, o, a.wide);
-                else st_raw<T, V>(out, o);
             }
         }
     }
@@ -268,6 +314,8 @@ static int32_t cache_side(const b200_tensor* Q, const b200_tensor* S, const char
     c->sh = S->stride[1]; c->sp = S->stride[2]; c->sn = S->stride[3];
     return B200_OK;
 }
+// The kernels take strides in 32 bits (and offsets in 64).
+static bool far(int64_t stride) { return stride > 0x7fffffff || stride < -0x7fffffff; }
 static int32_t cache_pair(const b200_tensor* KQ, const b200_tensor* KS, const b200_tensor* VQ, const b200_tensor* VS, CacheArgs* a) {
     B200_TRY(cache_side(KQ, KS, "cache keys", &a->k));
     B200_TRY(cache_side(VQ, VS, "cache values", &a->v));
@@ -276,6 +324,9 @@ static int32_t cache_pair(const b200_tensor* KQ, const b200_tensor* KS, const b2
     if (KQ->dtype != VQ->dtype) return fail(B200_INVALID_ARG, "cache: keys and values differ in format");
     if (KQ->shape[0] > 8192 || VQ->shape[0] > 8192 || KQ->shape[1] > 65536 || KQ->shape[2] > 0x3fffffff)
         return fail(B200_TOO_LARGE, "cache: heads of at most 8192 elements, 65536 heads, pages of at most 2^30-1 places");
+    for (const b200_tensor* t : {KQ, KS, VQ, VS})
+        if (far(t->stride[2]) || far(t->stride[3])) return fail(B200_TOO_LARGE, "cache: pages more than 2^31 bytes apart");
+    if (KQ->shape[3] > 0x7fffffff) return fail(B200_TOO_LARGE, "cache: at most 2^31-1 pages");
     a->heads = (int32_t)KQ->shape[1];
     a->page = (int32_t)KQ->shape[2];
     a->npages = KQ->shape[3];
@@ -359,9 +410,12 @@ extern "C" int32_t b200_cache_write(b200_stream_t st, const b200_tensor* KQ, con
     a.err = device_error_word(st->dev);
     auto fits = [&](int w) {
         return a.k.d % w == 0 && a.v.d % w == 0 && multiple_strides(K, w, 16) && multiple_strides(V, w, 16) &&
-               multiple_strides(KQ, w, (size_t)w) && multiple_strides(VQ, w, (size_t)w) && (a.half ? a.rot / 2 : a.rot) % w == 0;
+               multiple_strides(KQ, w, (size_t)w) && multiple_strides(VQ, w, (size_t)w);
     };
-    const int full = dtype == B200_F32 ? 8 : 16, v = fits(full) ? full : fits(full / 2) ? full / 2 : 1;
+    auto even = [&](int w) { return (a.half ? a.rot / 2 : a.rot) % w == 0; };
+    const int full = dtype == B200_F32 ? 8 : 16;
+    const int v = fits(full) && even(full) ? full : fits(full / 2) ? full / 2 : 1;
+    const bool uneven = v > 1 && !even(v);
     a.wide = multiple_strides(K, full, 32) && multiple_strides(V, full, 32) && (!a.half || a.rot / 2 % full == 0);
     a.per_page = FastDiv((uint32_t)a.page);
     for (CacheSide* s : {&a.k, &a.v}) {
@@ -387,7 +441,18 @@ extern "C" int32_t b200_cache_write(b200_stream_t st, const b200_tensor* KQ, con
     const size_t smem = (size_t)per_block * (a.rot / 2) * sizeof(float2);
     const unsigned grid = (unsigned)((a.tokens + per_block - 1) / per_block);
     B200_CUDA(by_row_type(dtype, v, [&](auto t, auto w) {
-        return launch_overlapped(cache_write_kernel<decltype(t), decltype(w)::value>, grid, 256u, smem, st->s, a);
+        using T = decltype(t);
+        constexpr int W = decltype(w)::value;
+        auto turn = [&](auto f) {
+            constexpr int F = decltype(f)::value;
+            if constexpr (W == 16 / (int)sizeof(T)) {
+                if (uneven) return launch_overlapped(cache_write_kernel<T, W, F, kTurnUneven>, grid, 256u, smem, st->s, a);
+            }
+            return a.rot == 0 ? launch_overlapped(cache_write_kernel<T, W, F, kNoTurn>, grid, 256u, smem, st->s, a)
+                   : a.half   ? launch_overlapped(cache_write_kernel<T, W, F, kTurnHalf>, grid, 256u, smem, st->s, a)
+                              : launch_overlapped(cache_write_kernel<T, W, F, kTurnInterleaved>, grid, 256u, smem, st->s, a);
+        };
+        return a.e4m3 ? turn(std::integral_constant<int, kE4M3>{}) : turn(std::integral_constant<int, kInt8>{});
     }));
     if (temp) B200_TRY(b200_free_async(temp, st));
     return finish(st, "b200_cache_write");
@@ -405,6 +470,8 @@ extern "C" int32_t b200_cache_read(b200_stream_t st, const b200_tensor* K, const
     if (K->shape[2] != V->shape[2] || K->shape[3] != V->shape[3]) return fail(B200_INVALID_ARG, "cache read: keys and values differ in places or sequences");
     a.places = K->shape[2];
     a.seqs = K->shape[3];
+    if (far(K->stride[2]) || far(V->stride[2]) || a.places > 0x3fffffff)
+        return fail(B200_TOO_LARGE, "cache read: at most 2^30 places, tokens at most 2^31 elements apart");
     B200_TRY(check_tensor(pages, "cache read pages"));
     if (!is_index_type(pages->dtype)) return fail(B200_UNSUPPORTED, "cache read: pages must be Int32 or Int64");
     if (pages->ndim != 2 || pages->shape[1] != a.seqs) return fail(B200_INVALID_ARG, "cache read: the page table is (pages of a sequence, sequences)");
@@ -428,24 +495,28 @@ extern "C" int32_t b200_cache_read(b200_stream_t st, const b200_tensor* K, const
         s->units = s->d / v * a.heads;
         s->per_head = FastDiv((uint32_t)(s->d / v));
     }
-    const int per_token = a.k.units + a.v.units, block = 256 * kReadUnroll;
+    const int per_token = a.k.units + a.v.units;
     a.per_token = FastDiv((uint32_t)per_token);
-    a.tile = per_token < block ? block / per_token : 1;
-    a.parts = (per_token + block - 1) / block;
-    if (a.places > 0x7fffffff - a.tile) return fail(B200_TOO_LARGE, "cache read: at most 2^31 places");
+    a.parts = (per_token + 255) / 256;
+    a.abreast = a.parts > 1 ? 1 : 256 / per_token;
+    a.tile = a.abreast * kReadUnroll * 2;
     int64_t bx = (a.places + a.tile - 1) / a.tile * a.parts;
     if (bx < 1) bx = 1;                                             // one block at least looks at the lengths
     if (bx > 0x7fffffff) return fail(B200_TOO_LARGE, "cache read: too many places for one call");
     const dim3 grid((unsigned)bx, (unsigned)(a.seqs < 65535 ? a.seqs : 65535));
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid;
-    cfg.blockDim = dim3(256);
+    cfg.blockDim = dim3((unsigned)(a.parts > 1 ? 256 : a.abreast * per_token));
     cfg.stream = st->s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = overlap_launches_enabled() ? 1 : 0;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    B200_CUDA(by_row_type(dtype, v, [&](auto t, auto w) { return cudaLaunchKernelEx(&cfg, cache_read_kernel<decltype(t), decltype(w)::value>, a); }));
+    B200_CUDA(by_row_type(dtype, v, [&](auto t, auto w) { 
+        using T = decltype(t);
+        constexpr int W = decltype(w)::value;
+        return a.e4m3 ? cudaLaunchKernelEx(&cfg, cache_read_kernel<T, W, kE4M3>, a) : cudaLaunchKernelEx(&cfg, cache_read_kernel<T, W, kInt8>, a);
+    }));
     return finish(st, "b200_cache_read");
 }

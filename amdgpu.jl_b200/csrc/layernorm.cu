@@ -276,7 +276,7 @@ norm_backward_kernel(NormArgs a) {
 // 72 us; waiting for each row in turn the gradient takes 120 us.  A register spilled inside the loop costs
 // more than a second pass over it (20 bytes: 69 -> 84 us).
 
-enum { kAsIs = 0, kInt8 = 1, kE4M3 = 2 };   // form of the rows kept for the gradient
+enum { kAsIs = 0 };                     // form of the rows kept for the gradient: as they are, kInt8, kE4M3
 
 struct GroupBarrier {
     int id, threads;

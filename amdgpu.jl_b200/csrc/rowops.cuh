@@ -83,6 +83,8 @@ struct FastDiv {
 #endif
 };
 
+enum { kInt8 = 1, kE4M3 = 2 };          // formats as template arguments
+
 #ifdef __CUDACC__
 // ---- vectors of elements -------------------------------------------------------------------------
 template <int BYTES> struct RawOfBytes;
