@@ -10,10 +10,6 @@
 
 namespace b200 {
 
-constexpr int kNormThreads = 256;
-constexpr int kNormElems = 16;          // elements of a row per thread
-constexpr int kNormMaxGroup = 512;      // threads per row
-
 struct NormArgs {
     const void *x, *dy, *gamma, *beta;
     void *y;                            // forward: y; gradient: dx
@@ -24,7 +20,8 @@ struct NormArgs {
     // ring kernels: rows from one of a group's to its next, and that many rows of each array in elements
     int64_t step, x_step, y_step, dy_step, q_step;
     float eps;
-    int32_t gamma_f32, e4m3, group;     // group: threads per row, a power of two
+    int32_t gamma_f32, e4m3, group;     // group: threads per row
+    int32_t pitch, pitch_x;             // rows of any alignment: bytes of a stage of the rings
 };
 
 __device__ __forceinline__ float load_param(const void* p, bool f32, int32_t dtype, int64_t i) {
@@ -41,225 +38,6 @@ __device__ __forceinline__ float lane_sum(float v, int width) {
 #pragma unroll
     for (int o = 16; o > 0; o /= 2) if (o < width) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
-}
-
-// ---- rows of any alignment ------------------------------------------------------------------------
-// `group` threads hold one row, element by element, so a row is read once; a block of kNormThreads (or one
-// group, if that is larger) works on several rows side by side and walks over the rows with the grid's
-// stride.
-//
-// Moments in one exchange: every warp takes the mean of its share and the squares about that mean;
-// the shares combine as M2 = sum M2_w + n_w (mean_w - mean)^2 (Chan, Golub and LeVeque 1983), which
-// loses nothing when the mean is large against the spread.
-template <typename T, int V, int NV, bool KEEP>
-__global__ void __launch_bounds__(kNormMaxGroup)
-norm_forward_kernel(NormArgs a) {
-    __shared__ float2 share[2][kNormMaxGroup / 32];
-    grid_dependency_wait();
-    const int G = a.group, group = threadIdx.x / G, t = threadIdx.x % G;
-    const int per_block = blockDim.x / G, warps = G / 32, warp = t / 32;
-    const int width = G < 32 ? G : 32;
-    const int nvec = (int)(a.d / V);
-    const T* x = reinterpret_cast<const T*>(a.x);
-    T* y = reinterpret_cast<T*>(a.y);
-
-    float gm[NV * V], bt[NV * V];
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-        const int vi = t + k * G;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            gm[k * V + i] = a.gamma && vi < nvec ? load_param(a.gamma, a.gamma_f32, dtype_of<T>(), (int64_t)vi * V + i) : 1.f;
-            bt[k * V + i] = a.beta && vi < nvec ? load_param(a.beta, a.gamma_f32, dtype_of<T>(), (int64_t)vi * V + i) : 0.f;
-        }
-    }
-    // elements of this warp's share of a row
-    int count = 0;
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-        const int left = nvec - (k * G + warp * 32);
-        count += (left < 0 ? 0 : left > width ? width : left) * V;
-    }
-    int parity = 0;
-    for (int64_t base = (int64_t)blockIdx.x * per_block; base < a.rows; base += (int64_t)gridDim.x * per_block) {
-        const int64_t row = base + group;
-        const bool live = row < a.rows;
-        float v[NV * V];
-        float sum = 0.f;
-#pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            const int vi = t + k * G;
-            RawVec<T, V> r{};
-            if (live && vi < nvec) r = ld_raw<T, V>(x + row * a.ldx + (int64_t)vi * V);
-            unpack<T, V>(r, v + k * V);
-        }
-#pragma unroll
-        for (int i = 0; i < NV * V; ++i) sum += v[i];
-        sum = lane_sum(sum, width);
-        float mean = count ? sum / (float)count : 0.f, m2 = 0.f;
-#pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            if (t + k * G < nvec) {
-#pragma unroll
-                for (int i = 0; i < V; ++i) { const float c = v[k * V + i] - mean; m2 = fmaf(c, c, m2); }
-            }
-        }
-        m2 = lane_sum(m2, width);
-        if (warps > 1) {
-            // a group has whole warps here and is the block or a power-of-two part of it
-            float2* sh = share[parity] + group * warps;
-            if ((t & 31) == 0) sh[warp] = make_float2(sum, m2);
-            __syncthreads();
-            parity ^= 1;
-            float total = 0.f;
-            for (int w = 0; w < warps; ++w) total += sh[w].x;
-            mean = total / (float)a.d;
-            m2 = 0.f;
-            for (int w = 0; w < warps; ++w) {
-                int n = 0;
-#pragma unroll
-                for (int k = 0; k < NV; ++k) {
-                    const int left = nvec - (k * G + w * 32);
-                    n += (left < 0 ? 0 : left > 32 ? 32 : left) * V;
-                }
-                if (n) { const float c = sh[w].x / (float)n - mean; m2 += sh[w].y + (float)n * c * c; }
-            }
-        }
-        const float rstd = 1.f / sqrtf(m2 / (float)a.d + a.eps);
-        if (live && t == 0) {
-            if (a.mean) a.mean[row] = mean;
-            if (a.rstd) a.rstd[row] = rstd;
-        }
-#pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            const int vi = t + k * G;
-            const bool in = live && vi < nvec;
-            float o[V];
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                v[k * V + i] = in ? (v[k * V + i] - mean) * rstd : 0.f;
-                o[i] = fmaf(v[k * V + i], gm[k * V + i], bt[k * V + i]);
-            }
-            if (in) st_raw<T, V>(y + row * a.ldy + (int64_t)vi * V, pack<T, V>(o));
-            if constexpr (KEEP) {
-                const uint32_t e = scale_byte(block_amax<V>(v + k * V), a.e4m3);
-                if (in) {
-                    st_raw<uint8_t, V>(a.q + row * a.d + (int64_t)vi * V, encode<V>(v + k * V, e, a.e4m3));
-                    if (vi % (kBlock / V) == 0) a.s[row * a.blocks + vi / (kBlock / V)] = (uint8_t)e;
-                }
-            }
-        }
-    }
-}
-
-template <typename T, int V, int NV, bool KEPT>
-__global__ void __launch_bounds__(kNormMaxGroup)
-norm_backward_kernel(NormArgs a) {
-    __shared__ float2 share[2][kNormMaxGroup / 32];
-    extern __shared__ float column[];   // [2][d] when several rows share the block
-    grid_dependency_wait();
-    const int G = a.group, group = threadIdx.x / G, t = threadIdx.x % G;
-    const int per_block = blockDim.x / G, warps = G / 32, warp = t / 32;
-    const int width = G < 32 ? G : 32;
-    const int nvec = (int)(a.d / V);
-    const T* x = reinterpret_cast<const T*>(a.x);
-    const T* dy = reinterpret_cast<const T*>(a.dy);
-    T* dx = reinterpret_cast<T*>(a.y);
-
-    float gm[NV * V], dg[NV * V], db[NV * V];
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-        const int vi = t + k * G;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            gm[k * V + i] = a.gamma && vi < nvec ? load_param(a.gamma, a.gamma_f32, dtype_of<T>(), (int64_t)vi * V + i) : 1.f;
-            dg[k * V + i] = db[k * V + i] = 0.f;
-        }
-    }
-    int parity = 0;
-    for (int64_t base = (int64_t)blockIdx.x * per_block; base < a.rows; base += (int64_t)gridDim.x * per_block) {
-        const int64_t row = base + group;
-        const bool live = row < a.rows;
-        const float rstd = live ? a.rstd[row] : 0.f;
-        const float mean = !KEPT && live ? a.mean[row] : 0.f;
-        float h[NV * V], g[NV * V];
-        float s1 = 0.f, s2 = 0.f;
-#pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            const int vi = t + k * G;
-            const bool in = live && vi < nvec;
-            RawVec<T, V> r{};
-            if (in) r = ld_raw<T, V>(dy + row * a.lddy + (int64_t)vi * V);
-            unpack<T, V>(r, g + k * V);
-            if constexpr (KEPT) {
-                RawVec<uint8_t, V> c{};
-                uint32_t e = 0;
-                if (in) {
-                    c = ld_raw<uint8_t, V>(a.q + row * a.d + (int64_t)vi * V);
-                    e = a.s[row * a.blocks + vi / (kBlock / V)];
-                }
-                decode<V>(c, e, a.e4m3, h + k * V);
-            } else {
-                r = RawVec<T, V>{};
-                if (in) r = ld_raw<T, V>(x + row * a.ldx + (int64_t)vi * V);
-                unpack<T, V>(r, h + k * V);
-            }
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const int j = k * V + i;
-                if constexpr (!KEPT) h[j] = in ? (h[j] - mean) * rstd : 0.f;
-                if (!in) h[j] = 0.f;
-                dg[j] = fmaf(g[j], h[j], dg[j]);
-                db[j] += g[j];
-                g[j] *= gm[j];
-                s1 += g[j];
-                s2 = fmaf(g[j], h[j], s2);
-            }
-        }
-        s1 = lane_sum(s1, width);
-        s2 = lane_sum(s2, width);
-        if (warps > 1) {
-            float2* sh = share[parity] + group * warps;
-            if ((t & 31) == 0) sh[warp] = make_float2(s1, s2);
-            __syncthreads();
-            parity ^= 1;
-            s1 = s2 = 0.f;
-            for (int w = 0; w < warps; ++w) { s1 += sh[w].x; s2 += sh[w].y; }
-        }
-        const float c1 = s1 / (float)a.d, c2 = s2 / (float)a.d;
-        if (dx) {
-#pragma unroll
-            for (int k = 0; k < NV; ++k) {
-                const int vi = t + k * G;
-                float o[V];
-#pragma unroll
-                for (int i = 0; i < V; ++i) o[i] = rstd * (g[k * V + i] - fmaf(h[k * V + i], c2, c1));
-                if (live && vi < nvec) st_raw<T, V>(dx + row * a.ldy + (int64_t)vi * V, pack<T, V>(o));
-            }
-        }
-    }
-    if (!a.partial) return;
-    float* out = a.partial + (int64_t)blockIdx.x * 2 * a.d;
-    // rows of one block, group after group, so that the order of the sum is fixed
-    for (int gi = 0; gi < per_block; ++gi) {
-        if (gi == group) {
-#pragma unroll
-            for (int k = 0; k < NV; ++k) {
-                const int vi = t + k * G;
-                if (vi < nvec) {
-#pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        const int64_t c = (int64_t)vi * V + i;
-                        float u = dg[k * V + i], w = db[k * V + i];
-                        if (gi > 0) { u += column[c]; w += column[a.d + c]; }
-                        if (gi + 1 < per_block) { column[c] = u; column[a.d + c] = w; }
-                        else { out[c] = u; out[a.d + c] = w; }
-                    }
-                }
-            }
-        }
-        if (per_block > 1) __syncthreads();
-    }
 }
 
 // ---- rows through a ring in shared memory -----------------------------------------------------------
@@ -672,6 +450,217 @@ norm_backward_ring_kernel(NormArgs a) {
     }
 }
 
+// ---- rows of any alignment ------------------------------------------------------------------------
+// The same for rows that start anywhere (odd widths, views): the aligned 16-byte pieces that cover a row go
+// through the ring, and a thread picks its columns t, t + group, ... out of them one by one, so its gamma and
+// its column sums stay its own whatever a row's offset.  The pieces are shared by a group: one more barrier
+// per row.  Pieces that reach past the first or the last byte of the array are copied element by element.
+constexpr int kAnyElems = 16;
+constexpr int kAnyStages = 3;
+constexpr int kAnyThreads = 512;
+
+template <typename T>
+struct PieceRing {
+    const char *lo, *hi;                       // the array's first byte and the one behind its last
+    char* buf;                                 // this group's first stage
+    int pitch, bytes;                          // of a stage; of a row
+    int64_t ld;
+    __device__ __forceinline__ PieceRing(const void* p, int64_t row_elems, int64_t ld_elems, int64_t rows, char* smem, int pitch_)
+        : lo(reinterpret_cast<const char*>(p)), hi(lo + ((rows - 1) * ld_elems + row_elems) * (int64_t)sizeof(T)), buf(smem), pitch(pitch_),
+          bytes((int)(row_elems * sizeof(T))), ld(ld_elems * (int64_t)sizeof(T)) {}
+    __device__ __forceinline__ int offset(int64_t row) const { return (int)(reinterpret_cast<uintptr_t>(lo + row * ld) & 15); }
+    __device__ __forceinline__ void fetch(int64_t row, int stage, int t, int G) const {
+        const char* first = lo + row * ld;
+        const char* from = first - offset(row);
+        char* to = buf + stage * pitch;
+        const int n = (offset(row) + bytes + 15) / 16;
+        for (int c = t; c < n; c += G) {
+            const char* src = from + 16 * c;
+            if (src >= lo && src + 16 <= hi) {
+                ring_copy<16>(to + 16 * c, src);
+            } else {
+                for (int j = 0; j < 16; j += (int)sizeof(T))
+                    if (src + j >= first && src + j < first + bytes) *reinterpret_cast<T*>(to + 16 * c + j) = *reinterpret_cast<const T*>(src + j);
+            }
+        }
+    }
+    __device__ __forceinline__ const T* row(int64_t r, int stage) const { return reinterpret_cast<const T*>(buf + stage * pitch + offset(r)); }
+};
+inline int piece_pitch(int64_t row_bytes) { return (int)((row_bytes + 15) / 16 * 16 + 16); }
+
+__device__ __forceinline__ void group_sync(const RingPlace& p) {
+    if (p.warps > 1) p.bar.sync();
+    else __syncwarp();
+}
+
+template <typename T, bool KEEP>
+__global__ void __launch_bounds__(kAnyThreads)
+norm_forward_any_kernel(NormArgs a) {
+    constexpr int E = kAnyElems;
+    extern __shared__ char pieces[];
+    __shared__ __align__(16) float shares[kAnyThreads / 64][4][kShare];
+    for (int i = threadIdx.x; i < (int)(sizeof(shares) / 4); i += blockDim.x) (&shares[0][0][0])[i] = 0.f;
+    __syncthreads();
+    grid_dependency_wait();
+    const RingPlace p(a.group, a.rows, a.step);
+    const int G = a.group, t = p.t, d = (int)a.d;
+    const PieceRing<T> ring(a.x, a.d, a.ldx, a.rows, pieces + p.group * kAnyStages * a.pitch, a.pitch);
+#pragma unroll
+    for (int s = 0; s < kAnyStages - 1; ++s) {
+        if (s < p.mine) ring.fetch(p.row + s * a.step, s, t, G);
+        cp_async_commit();
+    }
+    float gm[E], bt[E];
+#pragma unroll
+    for (int k = 0; k < E; ++k) {
+        const int c = t + k * G;
+        gm[k] = a.gamma && c < d ? load_param(a.gamma, a.gamma_f32, dtype_of<T>(), c) : 1.f;
+        bt[k] = a.beta && c < d ? load_param(a.beta, a.gamma_f32, dtype_of<T>(), c) : 0.f;
+    }
+    const float per_d = 1.f / (float)a.d;
+    float* share = &shares[p.warps > 1 ? p.group : 0][0][0];
+    int stage = 0;
+    int64_t row = p.row;
+    for (int it = 0; it < p.mine; ++it, row += a.step) {
+        cp_async_wait<kAnyStages - 2>();
+        group_sync(p);
+        const T* x = ring.row(row, stage);
+        float v[E];
+        float sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < E; ++k) v[k] = t + k * G < d ? Elem<T>::get(x[t + k * G]) : 0.f;
+        if (it + kAnyStages - 1 < p.mine) ring.fetch(row + (kAnyStages - 1) * a.step, stage == 0 ? kAnyStages - 1 : stage - 1, t, G);
+        cp_async_commit();
+        stage = stage + 1 == kAnyStages ? 0 : stage + 1;
+#pragma unroll
+        for (int k = 0; k < E; ++k) sum += v[k];
+        const float mean = group_sum(sum, p, share) * per_d;
+        float m2 = 0.f;
+#pragma unroll
+        for (int k = 0; k < E; ++k) {
+            v[k] = t + k * G < d ? v[k] - mean : 0.f;
+            m2 = fmaf(v[k], v[k], m2);
+        }
+        const float rstd = 1.f / sqrtf(fmaf(group_sum(m2, p, share + kShare), per_d, a.eps));
+        share = (it & 1) ? share - 2 * kShare : share + 2 * kShare;
+        if (t == 0) {
+            if (a.mean) a.mean[row] = mean;
+            if (a.rstd) a.rstd[row] = rstd;
+        }
+        T* y = reinterpret_cast<T*>(a.y) + row * a.ldy + t;
+#pragma unroll
+        for (int k = 0; k < E; ++k) {
+            v[k] *= rstd;
+            if (t + k * G < d) y[k * G] = Elem<T>::put(fmaf(v[k], gm[k], bt[k]));
+        }
+        if constexpr (KEEP) {
+            // a warp's columns t + k G are one block of 32; magnitudes compare like their bits, NaN above all
+            uint8_t *q = a.q + row * a.d + t, *sc = a.s + row * a.blocks + t / kBlock;
+#pragma unroll
+            for (int k = 0; k < E; ++k) {
+                if ((t & ~31) + k * G >= d) break;
+                const uint32_t e = scale_byte(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v[k]) & 0x7fffffffu)), a.e4m3);
+                if (t + k * G < d) q[k * G] = encode<1>(v + k, e, a.e4m3);
+                if (p.lane == 0) sc[k * G / kBlock] = (uint8_t)e;
+            }
+        }
+    }
+}
+
+template <typename T, bool KEPT>
+__global__ void __launch_bounds__(kAnyThreads)
+norm_backward_any_kernel(NormArgs a) {
+    constexpr int E = kAnyElems;
+    extern __shared__ char pieces[];                      // [group][stage]: dy, then of all groups x or codes
+    __shared__ __align__(16) float2 shares[kAnyThreads / 64][2][kShare];
+    for (int i = threadIdx.x; i < (int)(sizeof(shares) / 8); i += blockDim.x) (&shares[0][0][0])[i] = make_float2(0.f, 0.f);
+    __syncthreads();
+    grid_dependency_wait();
+    const RingPlace p(a.group, a.rows, a.step);
+    const int G = a.group, t = p.t, d = (int)a.d, per_block = blockDim.x / G;
+    using S = typename std::conditional<KEPT, uint8_t, T>::type;
+    char* second = pieces + per_block * kAnyStages * a.pitch;
+    const PieceRing<T> ring(a.dy, a.d, a.lddy, a.rows, pieces + p.group * kAnyStages * a.pitch, a.pitch);
+    const PieceRing<S> ring_x(KEPT ? (const void*)a.q : a.x, a.d, KEPT ? a.d : a.ldx, a.rows, second + p.group * kAnyStages * a.pitch_x, a.pitch_x);
+#pragma unroll
+    for (int s = 0; s < kAnyStages - 1; ++s) {
+        if (s < p.mine) { ring.fetch(p.row + s * a.step, s, t, G); ring_x.fetch(p.row + s * a.step, s, t, G); }
+        cp_async_commit();
+    }
+    float gm[E], dg[E], db[E];
+#pragma unroll
+    for (int k = 0; k < E; ++k) {
+        const int c = t + k * G;
+        gm[k] = a.gamma && c < d ? load_param(a.gamma, a.gamma_f32, dtype_of<T>(), c) : 1.f;
+        dg[k] = db[k] = 0.f;
+    }
+    const float per_d = 1.f / (float)a.d;
+    float2* share = &shares[p.warps > 1 ? p.group : 0][0][0];
+    int stage = 0;
+    int64_t row = p.row;
+    for (int it = 0; it < p.mine; ++it, row += a.step) {
+        const float rstd = a.rstd[row], mean = KEPT ? 0.f : a.mean[row];
+        const uint8_t* sc = a.s + row * a.blocks + t / kBlock;
+        cp_async_wait<kAnyStages - 2>();
+        group_sync(p);
+        const T* dy = ring.row(row, stage);
+        const S* x = ring_x.row(row, stage);
+        float g[E], h[E];
+        float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+        for (int k = 0; k < E; ++k) {
+            const int c = t + k * G;
+            g[k] = h[k] = 0.f;
+            if (c < d) {
+                g[k] = Elem<T>::get(dy[c]);
+                if constexpr (KEPT) decode<1>(x[c], sc[k * G / kBlock], a.e4m3, h + k);
+                else h[k] = (Elem<T>::get(x[c]) - mean) * rstd;
+            }
+            dg[k] = fmaf(g[k], h[k], dg[k]);
+            db[k] += g[k];
+            g[k] *= gm[k];
+            s1 += g[k];
+            s2 = fmaf(g[k], h[k], s2);
+        }
+        if (it + kAnyStages - 1 < p.mine) {
+            ring.fetch(row + (kAnyStages - 1) * a.step, stage == 0 ? kAnyStages - 1 : stage - 1, t, G);
+            ring_x.fetch(row + (kAnyStages - 1) * a.step, stage == 0 ? kAnyStages - 1 : stage - 1, t, G);
+        }
+        cp_async_commit();
+        stage = stage + 1 == kAnyStages ? 0 : stage + 1;
+        const float2 s = group_sum2(s1, s2, p, share);
+        share = (it & 1) ? share - kShare : share + kShare;
+        if (a.y) {
+            const float c1 = -s.x * per_d * rstd, c2 = -s.y * per_d * rstd;
+            T* dx = reinterpret_cast<T*>(a.y) + row * a.ldy + t;
+#pragma unroll
+            for (int k = 0; k < E; ++k)
+                if (t + k * G < d) dx[k * G] = Elem<T>::put(fmaf(h[k], c2, fmaf(g[k], rstd, c1)));
+        }
+    }
+    grid_dependency_release();
+    if (!a.partial) return;
+    // column sums as in the kernel above: groups side by side, joined in their order
+    float* column = reinterpret_cast<float*>(pieces);
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < E; ++k) {
+        const int c = t + k * G;
+        if (c < d) {
+            column[p.group * 2 * d + c] = dg[k];
+            column[p.group * 2 * d + d + c] = db[k];
+        }
+    }
+    __syncthreads();
+    float* out = a.partial + (int64_t)blockIdx.x * 2 * d;
+    for (int c = threadIdx.x; c < 2 * d; c += blockDim.x) {
+        float sum = column[c];
+#pragma unroll 4
+        for (int g = 1; g < per_block; ++g) sum += column[g * 2 * d + c];
+        out[c] = sum;
+    }
+}
+
 // Sums the partials: 4 W columns per block (W lanes of four), 1024 / W strands of partials, joined in a
 // fixed order.  VEC: d is a multiple of 4, so four columns are one access.
 template <bool VEC>
@@ -842,12 +831,6 @@ static int ring_group(int64_t d, int e, int v) {
     while (g < need) g *= 2;
     return g;
 }
-// Threads per row of the element kernels, 16 elements each: a power of two.
-static int norm_group(int64_t d) {
-    int g = 32;
-    while ((int64_t)g * kNormElems < d) g *= 2;
-    return g;
-}
 static int norm_vector(const NormArgs& a, int32_t dtype, bool aligned) {
     const int v = dtype == B200_F32 ? 4 : 8;
     return aligned && a.d % v == 0 && a.rows <= 0x3fffffff ? v : 1;    // the ring kernels count rows in 32 bits
@@ -901,12 +884,16 @@ static cudaError_t run_forward(b200_stream_t st, NormArgs a, int v) {
         a.group = ring_group(a.d, 32, v);
         if (a.group <= 256) return forward_ring<T, 32, 3, 256>(st, a);
         if (a.group <= 512) return forward_ring<T, 32, 3, 512>(st, a);
-    } else {
-        a.group = norm_group(a.d);
-        if (a.group <= kNormMaxGroup) {
+    } else if (a.rows <= 0x3fffffff) {
+        a.group = ring_group(a.d, kAnyElems, 1);
+        if (a.group <= kAnyThreads) {
             NormLaunch l{st, a};
-            auto run = [&](auto kernel) { const cudaError_t e = l.plan(kernel, a.group >= kNormThreads ? 1 : kNormThreads / a.group, 0); return e == cudaSuccess ? l.go(kernel) : e; };
-            return a.q ? run(norm_forward_kernel<T, 1, kNormElems, true>) : run(norm_forward_kernel<T, 1, kNormElems, false>);
+            l.a.pitch = piece_pitch(a.d * (int64_t)sizeof(T));
+            // blocks of 256 threads where a row needs no more: several to an SM
+            const int per = a.group >= 256 ? 1 : 256 / a.group;
+            const size_t bytes = (size_t)per * kAnyStages * l.a.pitch;
+            auto run = [&](auto kernel) { const cudaError_t e = l.plan(kernel, per, bytes); return e == cudaSuccess ? l.go(kernel) : e; };
+            return a.q ? run(norm_forward_any_kernel<T, true>) : run(norm_forward_any_kernel<T, false>);
         }
     }
     return launch_overlapped(norm_forward_long_kernel<T>, balanced_grid(a.rows, (int64_t)sm_count(st->dev) * 2), 1024u, 0, st->s, a);
@@ -980,16 +967,20 @@ static int32_t run_backward(b200_stream_t st, NormArgs a, int v, void* dgamma, v
             else if (a.q) B200_TRY((backward_ring<T, 32, 2, 512, kInt8, false>(l, room)));
             else B200_TRY((backward_ring<T, 32, 2, 512, kAsIs, false>(l, room)));
         }
-    } else if (v == 1 && norm_group(a.d) <= kNormMaxGroup) {
-        l.a.group = norm_group(a.d);
-        const int per = l.a.group >= kNormThreads ? 1 : kNormThreads / l.a.group;
+    } else if (v == 1 && a.rows <= 0x3fffffff && ring_group(a.d, kAnyElems, 1) <= kAnyThreads) {
+        l.a.group = ring_group(a.d, kAnyElems, 1);
+        l.a.pitch = piece_pitch(a.d * (int64_t)sizeof(T));
+        l.a.pitch_x = piece_pitch(a.q ? a.d : a.d * (int64_t)sizeof(T));
+        const int per = kAnyThreads / l.a.group;
+        size_t bytes = (size_t)per * kAnyStages * (l.a.pitch + l.a.pitch_x);
+        if (bytes < (size_t)per * 2 * a.d * sizeof(float)) bytes = (size_t)per * 2 * a.d * sizeof(float);
         auto run = [&](auto kernel) -> int32_t {
-            B200_CUDA(l.plan(kernel, per, per > 1 ? 2 * a.d * sizeof(float) : 0));
+            B200_CUDA(l.plan(kernel, per, bytes));
             B200_TRY(room(l.grid));
             B200_CUDA(l.go(kernel));
             return B200_OK;
         };
-        B200_TRY(a.q ? run(norm_backward_kernel<T, 1, kNormElems, true>) : run(norm_backward_kernel<T, 1, kNormElems, false>));
+        B200_TRY(a.q ? run(norm_backward_any_kernel<T, true>) : run(norm_backward_any_kernel<T, false>));
     } else {
         const int64_t tiles = (a.d + 31) / 32;
         int64_t n = (int64_t)sm_count(st->dev) * 8 / tiles;
