@@ -21,7 +21,7 @@ struct NormArgs {
     int64_t step, x_step, y_step, dy_step, q_step;
     float eps;
     int32_t gamma_f32, e4m3, group;     // group: threads per row
-    int32_t pitch, pitch_x;             // rows of any alignment: bytes of a stage of the rings
+    int32_t pitch, pitch_x, units2;     // rows of any alignment: bytes of a stage of the rings; two elements at a time
 };
 
 __device__ __forceinline__ float load_param(const void* p, bool f32, int32_t dtype, int64_t i) {
@@ -493,30 +493,87 @@ __device__ __forceinline__ void group_sync(const RingPlace& p) {
     else __syncwarp();
 }
 
-template <typename T, bool KEEP>
-__global__ void __launch_bounds__(kAnyThreads)
+// A thread's columns: units of W neighbours, its warp's first unit + lane + 32 k for k < count (steps known
+// at compile time: no registers for addresses); W is 2 where every row of 16-bit elements starts on 4 bytes.
+// Two elements to a pair: those of a unit, or those of units 2j, 2j+1.
+template <int W>
+struct AnyColumns {
+    static constexpr int NU = kAnyElems / W;
+    int unit, count;
+    __device__ __forceinline__ AnyColumns(int t, int d) : unit(t / 32 * 32 * NU + t % 32) {
+        const int units = d / W;
+        count = unit < units ? min(NU, (units - unit + 31) / 32) : 0;
+    }
+    __device__ __forceinline__ int column(int k) const { return (unit + 32 * k) * W; }
+    // pairs of a row in shared memory, zeros beyond the row
+    template <typename T>
+    __device__ __forceinline__ void load(const T* x, F2* v) const {
+#pragma unroll
+        for (int k = 0; k < NU; ++k) {
+            RawVec<T, W> r{};
+            if (k < count) r = *reinterpret_cast<const RawVec<T, W>*>(x + unit * W + 32 * W * k);
+            float f[2];
+            unpack<T, W>(r, f);
+            put(v, k, f);
+        }
+    }
+    __device__ __forceinline__ void put(F2* v, int k, const float* f) const {
+        if constexpr (W == 2) v[k] = f2(f[0], f[1]);
+        else v[k / 2] = k & 1 ? f2(f2_parts(v[k / 2]).x, f[0]) : f2(f[0], 0.f);
+    }
+    __device__ __forceinline__ void get(const F2* v, int k, float* f) const {
+        const float2 x = f2_parts(v[k * W / 2]);
+        if constexpr (W == 2) { f[0] = x.x; f[1] = x.y; }
+        else f[0] = k & 1 ? x.y : x.x;
+    }
+    template <typename T>
+    __device__ __forceinline__ void store(T* y, const F2* v) const {
+#pragma unroll
+        for (int k = 0; k < NU; ++k) {
+            float f[2];
+            get(v, k, f);
+            if (k < count) *reinterpret_cast<RawVec<T, W>*>(y + unit * W + 32 * W * k) = pack<T, W>(f);
+        }
+    }
+    // 1 in the columns of the row, 0 beyond
+    __device__ __forceinline__ F2 mask(int j) const {
+        if constexpr (W == 2) return f2(j < count ? 1.f : 0.f);
+        else return f2(2 * j < count ? 1.f : 0.f, 2 * j + 1 < count ? 1.f : 0.f);
+    }
+    template <typename T>
+    __device__ __forceinline__ void params(const NormArgs& a, const void* p, float missing, F2* v) const {
+#pragma unroll
+        for (int k = 0; k < NU; ++k) {
+            float f[2] = {missing, missing};
+            if (p && k < count) {
+#pragma unroll
+                for (int i = 0; i < W; ++i) f[i] = load_param(p, a.gamma_f32, dtype_of<T>(), column(k) + i);
+            }
+            put(v, k, f);
+        }
+    }
+};
+
+template <typename T, int W, int THREADS, bool KEEP>
+__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1)
 norm_forward_any_kernel(NormArgs a) {
     constexpr int E = kAnyElems;
     extern __shared__ char pieces[];
-    __shared__ __align__(16) float shares[kAnyThreads / 64][4][kShare];
+    __shared__ __align__(16) float shares[THREADS / 64][4][kShare];
     for (int i = threadIdx.x; i < (int)(sizeof(shares) / 4); i += blockDim.x) (&shares[0][0][0])[i] = 0.f;
     __syncthreads();
     grid_dependency_wait();
     const RingPlace p(a.group, a.rows, a.step);
-    const int G = a.group, t = p.t, d = (int)a.d;
+    const AnyColumns<W> mine(p.t, (int)a.d);
     const PieceRing<T> ring(a.x, a.d, a.ldx, a.rows, pieces + p.group * kAnyStages * a.pitch, a.pitch);
 #pragma unroll
     for (int s = 0; s < kAnyStages - 1; ++s) {
-        if (s < p.mine) ring.fetch(p.row + s * a.step, s, t, G);
+        if (s < p.mine) ring.fetch(p.row + s * a.step, s, p.t, a.group);
         cp_async_commit();
     }
-    float gm[E], bt[E];
-#pragma unroll
-    for (int k = 0; k < E; ++k) {
-        const int c = t + k * G;
-        gm[k] = a.gamma && c < d ? load_param(a.gamma, a.gamma_f32, dtype_of<T>(), c) : 1.f;
-        bt[k] = a.beta && c < d ? load_param(a.beta, a.gamma_f32, dtype_of<T>(), c) : 0.f;
-    }
+    F2 gm[E / 2], bt[E / 2];
+    mine.template params<T>(a, a.gamma, 1.f, gm);
+    mine.template params<T>(a, a.beta, 0.f, bt);
     const float per_d = 1.f / (float)a.d;
     float* share = &shares[p.warps > 1 ? p.group : 0][0][0];
     int stage = 0;
@@ -524,50 +581,64 @@ norm_forward_any_kernel(NormArgs a) {
     for (int it = 0; it < p.mine; ++it, row += a.step) {
         cp_async_wait<kAnyStages - 2>();
         group_sync(p);
-        const T* x = ring.row(row, stage);
-        float v[E];
-        float sum = 0.f;
-#pragma unroll
-        for (int k = 0; k < E; ++k) v[k] = t + k * G < d ? Elem<T>::get(x[t + k * G]) : 0.f;
-        if (it + kAnyStages - 1 < p.mine) ring.fetch(row + (kAnyStages - 1) * a.step, stage == 0 ? kAnyStages - 1 : stage - 1, t, G);
+        F2 v[E / 2];
+        mine.load(ring.row(row, stage), v);
+        if (it + kAnyStages - 1 < p.mine) ring.fetch(row + (kAnyStages - 1) * a.step, stage == 0 ? kAnyStages - 1 : stage - 1, p.t, a.group);
         cp_async_commit();
         stage = stage + 1 == kAnyStages ? 0 : stage + 1;
+        F2 sum = f2(0.f), m2 = f2(0.f);
 #pragma unroll
-        for (int k = 0; k < E; ++k) sum += v[k];
-        const float mean = group_sum(sum, p, share) * per_d;
-        float m2 = 0.f;
+        for (int j = 0; j < E / 2; ++j) sum = f2_add(sum, v[j]);
+        const float mean = group_sum(f2_total(sum), p, share) * per_d;
+        const F2 minus = f2(-mean);
 #pragma unroll
-        for (int k = 0; k < E; ++k) {
-            v[k] = t + k * G < d ? v[k] - mean : 0.f;
-            m2 = fmaf(v[k], v[k], m2);
+        for (int j = 0; j < E / 2; ++j) {
+            v[j] = f2_fma(minus, mine.mask(j), v[j]);     // beyond the row: zeros stay zeros
+            m2 = f2_fma(v[j], v[j], m2);
         }
-        const float rstd = 1.f / sqrtf(fmaf(group_sum(m2, p, share + kShare), per_d, a.eps));
+        const float rstd = 1.f / sqrtf(fmaf(group_sum(f2_total(m2), p, share + kShare), per_d, a.eps));
         share = (it & 1) ? share - 2 * kShare : share + 2 * kShare;
-        if (t == 0) {
+        if (p.t == 0) {
             if (a.mean) a.mean[row] = mean;
             if (a.rstd) a.rstd[row] = rstd;
         }
-        T* y = reinterpret_cast<T*>(a.y) + row * a.ldy + t;
+        const F2 r2 = f2(rstd);
+        F2 o[E / 2];
 #pragma unroll
-        for (int k = 0; k < E; ++k) {
-            v[k] *= rstd;
-            if (t + k * G < d) y[k * G] = Elem<T>::put(fmaf(v[k], gm[k], bt[k]));
+        for (int j = 0; j < E / 2; ++j) {
+            v[j] = f2_mul(v[j], r2);
+            o[j] = f2_fma(v[j], gm[j], bt[j]);
         }
+        mine.store(reinterpret_cast<T*>(a.y) + row * a.ldy, o);
         if constexpr (KEEP) {
-            // a warp's columns t + k G are one block of 32; magnitudes compare like their bits, NaN above all
-            uint8_t *q = a.q + row * a.d + t, *sc = a.s + row * a.blocks + t / kBlock;
+            // 32 / W neighbouring lanes hold a block of 32; magnitudes compare like their bits, NaN above all
+            uint8_t* q = a.q + row * a.d + mine.unit * W;
+            uint8_t* sc = a.s + row * a.blocks + mine.unit * W / kBlock;
 #pragma unroll
-            for (int k = 0; k < E; ++k) {
-                if ((t & ~31) + k * G >= d) break;
-                const uint32_t e = scale_byte(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v[k]) & 0x7fffffffu)), a.e4m3);
-                if (t + k * G < d) q[k * G] = encode<1>(v + k, e, a.e4m3);
-                if (p.lane == 0) sc[k * G / kBlock] = (uint8_t)e;
+            for (int k = 0; k < mine.NU; ++k) {
+                if (mine.column(k) - p.t % 32 * W >= (int)a.d) break;      // the same for the whole warp
+                float f[2] = {0.f, 0.f};
+                mine.get(v, k, f);
+                uint32_t m = __float_as_uint(f[0]) & 0x7fffffffu;
+                if constexpr (W == 2) {
+                    m = max(m, __float_as_uint(f[1]) & 0x7fffffffu);
+#pragma unroll
+                    for (int o = 8; o > 0; o /= 2) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+                } else {
+                    m = __reduce_max_sync(0xffffffffu, m);
+                }
+                const uint32_t e = scale_byte(__uint_as_float(m), a.e4m3);
+                if (k < mine.count) {
+                    if constexpr (W == 2) *reinterpret_cast<uint16_t*>(q + 32 * W * k) = (uint16_t)(encode<1>(f, e, a.e4m3) | encode<1>(f + 1, e, a.e4m3) << 8);
+                    else q[32 * k] = encode<1>(f, e, a.e4m3);
+                    if (p.t % (kBlock / W) == 0) sc[W * k] = (uint8_t)e;
+                }
             }
         }
     }
 }
 
-template <typename T, bool KEPT>
+template <typename T, int W, bool KEPT>
 __global__ void __launch_bounds__(kAnyThreads)
 norm_backward_any_kernel(NormArgs a) {
     constexpr int E = kAnyElems;
@@ -577,81 +648,93 @@ norm_backward_any_kernel(NormArgs a) {
     __syncthreads();
     grid_dependency_wait();
     const RingPlace p(a.group, a.rows, a.step);
-    const int G = a.group, t = p.t, d = (int)a.d, per_block = blockDim.x / G;
+    const int G = a.group, d = (int)a.d, per_block = blockDim.x / G;
+    const AnyColumns<W> mine(p.t, d);
     using S = typename std::conditional<KEPT, uint8_t, T>::type;
     char* second = pieces + per_block * kAnyStages * a.pitch;
     const PieceRing<T> ring(a.dy, a.d, a.lddy, a.rows, pieces + p.group * kAnyStages * a.pitch, a.pitch);
     const PieceRing<S> ring_x(KEPT ? (const void*)a.q : a.x, a.d, KEPT ? a.d : a.ldx, a.rows, second + p.group * kAnyStages * a.pitch_x, a.pitch_x);
 #pragma unroll
     for (int s = 0; s < kAnyStages - 1; ++s) {
-        if (s < p.mine) { ring.fetch(p.row + s * a.step, s, t, G); ring_x.fetch(p.row + s * a.step, s, t, G); }
+        if (s < p.mine) { ring.fetch(p.row + s * a.step, s, p.t, G); ring_x.fetch(p.row + s * a.step, s, p.t, G); }
         cp_async_commit();
     }
-    float gm[E], dg[E], db[E];
+    F2 gm[E / 2], dg[E / 2], db[E / 2];
+    mine.template params<T>(a, a.gamma, 1.f, gm);
 #pragma unroll
-    for (int k = 0; k < E; ++k) {
-        const int c = t + k * G;
-        gm[k] = a.gamma && c < d ? load_param(a.gamma, a.gamma_f32, dtype_of<T>(), c) : 1.f;
-        dg[k] = db[k] = 0.f;
-    }
+    for (int j = 0; j < E / 2; ++j) dg[j] = db[j] = f2(0.f);
     const float per_d = 1.f / (float)a.d;
     float2* share = &shares[p.warps > 1 ? p.group : 0][0][0];
-    int stage = 0;
-    int64_t row = p.row;
-    for (int it = 0; it < p.mine; ++it, row += a.step) {
+    int stage = 0, row = (int)p.row;
+    for (int it = 0; it < p.mine; ++it, row += (int)a.step) {
         const float rstd = a.rstd[row], mean = KEPT ? 0.f : a.mean[row];
-        const uint8_t* sc = a.s + row * a.blocks + t / kBlock;
         cp_async_wait<kAnyStages - 2>();
         group_sync(p);
-        const T* dy = ring.row(row, stage);
+        F2 g[E / 2], h[E / 2];
+        mine.load(ring.row(row, stage), g);
         const S* x = ring_x.row(row, stage);
-        float g[E], h[E];
-        float s1 = 0.f, s2 = 0.f;
+        if constexpr (KEPT) {
+            const uint8_t* sc = a.s + row * a.blocks + mine.unit * W / kBlock;
 #pragma unroll
-        for (int k = 0; k < E; ++k) {
-            const int c = t + k * G;
-            g[k] = h[k] = 0.f;
-            if (c < d) {
-                g[k] = Elem<T>::get(dy[c]);
-                if constexpr (KEPT) decode<1>(x[c], sc[k * G / kBlock], a.e4m3, h + k);
-                else h[k] = (Elem<T>::get(x[c]) - mean) * rstd;
+            for (int k = 0; k < mine.NU; ++k) {
+                float f[2] = {0.f, 0.f};
+                if (k < mine.count) {
+                    const uint32_t e = sc[W * k];
+#pragma unroll
+                    for (int i = 0; i < W; ++i) decode<1>(x[mine.unit * W + 32 * W * k + i], e, a.e4m3, f + i);
+                }
+                mine.put(h, k, f);
             }
-            dg[k] = fmaf(g[k], h[k], dg[k]);
-            db[k] += g[k];
-            g[k] *= gm[k];
-            s1 += g[k];
-            s2 = fmaf(g[k], h[k], s2);
+        } else {
+            mine.load(x, h);
+            const F2 minus = f2(-mean), r2 = f2(rstd);
+#pragma unroll
+            for (int j = 0; j < E / 2; ++j) h[j] = f2_mul(f2_fma(minus, mine.mask(j), h[j]), r2);
+        }
+        F2 s1 = f2(0.f), s2 = f2(0.f);
+#pragma unroll
+        for (int j = 0; j < E / 2; ++j) {
+            dg[j] = f2_fma(g[j], h[j], dg[j]);
+            db[j] = f2_add(db[j], g[j]);
+            g[j] = f2_mul(g[j], gm[j]);
+            s1 = f2_add(s1, g[j]);
+            s2 = f2_fma(g[j], h[j], s2);
         }
         if (it + kAnyStages - 1 < p.mine) {
-            ring.fetch(row + (kAnyStages - 1) * a.step, stage == 0 ? kAnyStages - 1 : stage - 1, t, G);
-            ring_x.fetch(row + (kAnyStages - 1) * a.step, stage == 0 ? kAnyStages - 1 : stage - 1, t, G);
+            const int next = row + (kAnyStages - 1) * (int)a.step, to = stage == 0 ? kAnyStages - 1 : stage - 1;
+            ring.fetch(next, to, p.t, G);
+            ring_x.fetch(next, to, p.t, G);
         }
         cp_async_commit();
         stage = stage + 1 == kAnyStages ? 0 : stage + 1;
-        const float2 s = group_sum2(s1, s2, p, share);
+        const float2 s = group_sum2(f2_total(s1), f2_total(s2), p, share);
         share = (it & 1) ? share - kShare : share + kShare;
         if (a.y) {
-            const float c1 = -s.x * per_d * rstd, c2 = -s.y * per_d * rstd;
-            T* dx = reinterpret_cast<T*>(a.y) + row * a.ldy + t;
+            const F2 c1 = f2(-s.x * per_d * rstd), c2 = f2(-s.y * per_d * rstd), r2 = f2(rstd);
 #pragma unroll
-            for (int k = 0; k < E; ++k)
-                if (t + k * G < d) dx[k * G] = Elem<T>::put(fmaf(h[k], c2, fmaf(g[k], rstd, c1)));
+            for (int j = 0; j < E / 2; ++j) g[j] = f2_fma(h[j], c2, f2_fma(g[j], r2, c1));
+            mine.store(reinterpret_cast<T*>(a.y) + row * a.ldy, g);
         }
     }
     grid_dependency_release();
     if (!a.partial) return;
     // column sums as in the kernel above: groups side by side, joined in their order
-    float* column = reinterpret_cast<float*>(pieces);
+    float* column = reinterpret_cast<float*>(pieces) + p.group * 2 * d;
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < E; ++k) {
-        const int c = t + k * G;
-        if (c < d) {
-            column[p.group * 2 * d + c] = dg[k];
-            column[p.group * 2 * d + d + c] = db[k];
+    for (int k = 0; k < mine.NU; ++k) {
+        float f[2];
+        if (k < mine.count) {
+            mine.get(dg, k, f);
+#pragma unroll
+            for (int i = 0; i < W; ++i) column[mine.column(k) + i] = f[i];
+            mine.get(db, k, f);
+#pragma unroll
+            for (int i = 0; i < W; ++i) column[d + mine.column(k) + i] = f[i];
         }
     }
     __syncthreads();
+    column = reinterpret_cast<float*>(pieces);
     float* out = a.partial + (int64_t)blockIdx.x * 2 * d;
     for (int c = threadIdx.x; c < 2 * d; c += blockDim.x) {
         float sum = column[c];
@@ -893,7 +976,13 @@ static cudaError_t run_forward(b200_stream_t st, NormArgs a, int v) {
             const int per = a.group >= 256 ? 1 : 256 / a.group;
             const size_t bytes = (size_t)per * kAnyStages * l.a.pitch;
             auto run = [&](auto kernel) { const cudaError_t e = l.plan(kernel, per, bytes); return e == cudaSuccess ? l.go(kernel) : e; };
-            return a.q ? run(norm_forward_any_kernel<T, true>) : run(norm_forward_any_kernel<T, false>);
+            auto width = [&](auto w) {
+                constexpr int W = decltype(w)::value;
+                if (a.group <= 256) return a.q ? run(norm_forward_any_kernel<T, W, 256, true>) : run(norm_forward_any_kernel<T, W, 256, false>);
+                return a.q ? run(norm_forward_any_kernel<T, W, 512, true>) : run(norm_forward_any_kernel<T, W, 512, false>);
+            };
+            if constexpr (sizeof(T) == 2) { if (a.units2) return width(std::integral_constant<int, 2>{}); }
+            return width(std::integral_constant<int, 1>{});
         }
     }
     return launch_overlapped(norm_forward_long_kernel<T>, balanced_grid(a.rows, (int64_t)sm_count(st->dev) * 2), 1024u, 0, st->s, a);
@@ -980,7 +1069,10 @@ static int32_t run_backward(b200_stream_t st, NormArgs a, int v, void* dgamma, v
             B200_CUDA(l.go(kernel));
             return B200_OK;
         };
-        B200_TRY(a.q ? run(norm_backward_any_kernel<T, true>) : run(norm_backward_any_kernel<T, false>));
+        if constexpr (k16) {
+            if (a.units2) B200_TRY(a.q ? run(norm_backward_any_kernel<T, 2, true>) : run(norm_backward_any_kernel<T, 2, false>));
+        }
+        if (!a.units2) B200_TRY(a.q ? run(norm_backward_any_kernel<T, 1, true>) : run(norm_backward_any_kernel<T, 1, false>));
     } else {
         const int64_t tiles = (a.d + 31) / 32;
         int64_t n = (int64_t)sm_count(st->dev) * 8 / tiles;
@@ -1058,6 +1150,7 @@ extern "C" int32_t b200_layernorm(b200_stream_t st, const b200_tensor* Y, const 
     a.rstd = rstd ? (float*)rstd->ptr : nullptr;
     if (Q) { a.q = (uint8_t*)Q->ptr; a.s = (uint8_t*)S->ptr; a.e4m3 = Q->dtype == B200_U8; a.blocks = row_blocks(x.d); }
     const int full = x.dtype == B200_F32 ? 4 : 8;
+    a.units2 = x.dtype != B200_F32 && x.d % 2 == 0 && rows_aligned(x, 4) && rows_aligned(y, 4) && (!Q || reinterpret_cast<uintptr_t>(a.q) % 2 == 0);
     const int v = norm_vector(a, x.dtype, rows_aligned(x, 16) && rows_aligned(y, 16) && (!Q || reinterpret_cast<uintptr_t>(a.q) % full == 0));
     switch (x.dtype) {
         case B200_F16: B200_CUDA(run_forward<__half>(st, a, v)); break;
@@ -1114,6 +1207,8 @@ extern "C" int32_t b200_layernorm_backward(b200_stream_t st, const b200_tensor* 
     a.rstd = (float*)rstd->ptr;
     if (Q) { a.q = (uint8_t*)Q->ptr; a.s = (uint8_t*)S->ptr; a.e4m3 = Q->dtype == B200_U8; a.blocks = row_blocks(dy.d); }
     const int full = dy.dtype == B200_F32 ? 4 : 8;
+    a.units2 = dy.dtype != B200_F32 && dy.d % 2 == 0 && rows_aligned(dy, 4) && (!dX || rows_aligned(dx, 4)) && (!X || rows_aligned(x, 4)) &&
+               (!Q || reinterpret_cast<uintptr_t>(a.q) % 2 == 0);
     const int v = norm_vector(a, dy.dtype, rows_aligned(dy, 16) && (!dX || rows_aligned(dx, 16)) && (!X || rows_aligned(x, 16)) &&
                                                (!Q || reinterpret_cast<uintptr_t>(a.q) % full == 0));
     void* dg = dgamma ? dgamma->ptr : nullptr;
