@@ -71,10 +71,10 @@ __device__ __forceinline__ void activate2(F2 a, F2& f, F2& df) {
     }
 }
 
-// ---- rows of whole 8-bit blocks ------------------------------------------------------------------
-// Rows dealt out as vectors of V elements, each row filled up to whole blocks so that the 32/V lanes
-// of a block are neighbours in one warp.  `flat`: the rows have no gaps and d is a multiple of 32, so
-// they are one long row and no index is divided.
+// ---- rows of any alignment --------------------------------------------------------------------------
+// Rows are dealt out as vectors of V elements, each row filled up to whole blocks so that the 32/V lanes of
+// a block are neighbours in one warp.  `flat`: the rows have no gaps and d is a multiple of 32, so they are
+// one long row and no index is divided.
 struct RowsArgs {
     const void *a, *b, *dy;
     void *y, *da, *db;
@@ -95,98 +95,142 @@ __device__ __forceinline__ Slot slot_of(const RowsArgs& a, int64_t n) {
     return s;
 }
 
-template <int V>
-__device__ __forceinline__ void keep(const RowsArgs& a, const Slot& s, const float* v, uint8_t* q, uint8_t* sc) {
-    const uint32_t e = scale_byte(block_amax<V>(v), a.e4m3);
-    if (!s.in) return;
-    st_raw<uint8_t, V>(q + s.row * a.d + s.i, encode<V>(v, e, a.e4m3));
-    if (s.i % kBlock == 0) sc[s.row * a.blocks + s.i / kBlock] = (uint8_t)e;
-}
+// One element per lane and block of 32, kAny blocks per warp whose loads are on their way together.
+constexpr int kAny = 8;
 
-template <typename T, int V>
-__global__ void __launch_bounds__(256)
-quantize_kernel(RowsArgs a) {
-    grid_dependency_wait();
-    const int64_t step = (int64_t)gridDim.x * blockDim.x;
-    for (int64_t n0 = (int64_t)blockIdx.x * blockDim.x; n0 < a.slots; n0 += step) {
-        const Slot s = slot_of<V>(a, n0 + threadIdx.x);
-        RawVec<T, V> r{};
-        if (s.in) r = ld_raw<T, V>(reinterpret_cast<const T*>(a.a) + s.row * a.lda + s.i);
-        float v[V];
-        unpack<T, V>(r, v);
-        keep<V>(a, s, v, a.qa, a.sa);
-    }
-}
-
-template <typename T, int V>
-__global__ void __launch_bounds__(256)
-dequantize_kernel(RowsArgs a) {
-    grid_dependency_wait();
-    const int64_t step = (int64_t)gridDim.x * blockDim.x;
-    for (int64_t n = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; n < a.slots; n += step) {
-        const Slot s = slot_of<V>(a, n);
-        if (!s.in) continue;
-        float v[V];
-        decode_as<T, V>(ld_raw<uint8_t, V>(a.qa + s.row * a.d + s.i), a.sa[s.row * a.blocks + s.i / kBlock], a.e4m3, v);
-        st_raw<T, V>(reinterpret_cast<T*>(a.y) + s.row * a.ldy + s.i, pack<T, V>(v));
-    }
-}
-
-template <typename T, int V, bool GATED>
-__global__ void __launch_bounds__(256)
-activation_kernel(RowsArgs a) {
-    grid_dependency_wait();
-    const int64_t step = (int64_t)gridDim.x * blockDim.x;
-    for (int64_t n0 = (int64_t)blockIdx.x * blockDim.x; n0 < a.slots; n0 += step) {
-        const Slot s = slot_of<V>(a, n0 + threadIdx.x);
-        RawVec<T, V> ra{}, rb{};
-        if (s.in) {
-            ra = ld_raw<T, V>(reinterpret_cast<const T*>(a.a) + s.row * a.lda + s.i);
-            if constexpr (GATED) rb = ld_raw<T, V>(reinterpret_cast<const T*>(a.b) + s.row * a.ldb + s.i);
-        }
-        float v[V], g[V], o[V];
-        unpack<T, V>(ra, v);
-        if constexpr (GATED) unpack<T, V>(rb, g);
+__device__ __forceinline__ void any_slots(const RowsArgs& a, Slot s[kAny]) {
+    const int64_t first = ((int64_t)blockIdx.x * 8 + threadIdx.x / 32) * kAny;      // the warp's first block
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            float df;
-            a.act == kSilu ? activate<kSilu>(v[i], o[i], df) : activate<kGelu>(v[i], o[i], df);
-            if constexpr (GATED) o[i] *= g[i];
-        }
-        if (s.in) st_raw<T, V>(reinterpret_cast<T*>(a.y) + s.row * a.ldy + s.i, pack<T, V>(o));
-        if (a.qa) keep<V>(a, s, v, a.qa, a.sa);
-        if constexpr (GATED) { if (a.qb) keep<V>(a, s, g, a.qb, a.sb); }
+    for (int k = 0; k < kAny; ++k) s[k] = slot_of<1>(a, (first + k) * kBlock + threadIdx.x % 32);
+}
+template <typename T>
+__device__ __forceinline__ void any_load(const void* p, int64_t ld, const Slot s[kAny], float* v) {
+    T r[kAny];
+#pragma unroll
+    for (int k = 0; k < kAny; ++k) {
+        r[k] = Elem<T>::put(0.f);
+        if (s[k].in) r[k] = reinterpret_cast<const T*>(p)[s[k].row * ld + s[k].i];
+    }
+#pragma unroll
+    for (int k = 0; k < kAny; ++k) v[k] = Elem<T>::get(r[k]);
+}
+template <typename T>
+__device__ __forceinline__ void any_store(void* p, int64_t ld, const Slot s[kAny], const float* v) {
+#pragma unroll
+    for (int k = 0; k < kAny; ++k) if (s[k].in) reinterpret_cast<T*>(p)[s[k].row * ld + s[k].i] = Elem<T>::put(v[k]);
+}
+// Magnitudes compare like their bits, NaN above all.
+__device__ __forceinline__ void any_keep(const RowsArgs& a, const Slot s[kAny], const float* v, uint8_t* q, uint8_t* sc) {
+#pragma unroll
+    for (int k = 0; k < kAny; ++k) {
+        const uint32_t m = __reduce_max_sync(0xffffffffu, s[k].in ? __float_as_uint(v[k]) & 0x7fffffffu : 0u);
+        const uint32_t e = scale_byte(__uint_as_float(m), a.e4m3);
+        if (!s[k].in) continue;
+        q[s[k].row * a.d + s[k].i] = encode<1>(v + k, e, a.e4m3);
+        if (threadIdx.x % 32 == 0) sc[s[k].row * a.blocks + s[k].i / kBlock] = (uint8_t)e;
     }
 }
-
-template <typename T, int V, bool GATED, bool KEPT>
-__global__ void __launch_bounds__(256)
-activation_backward_kernel(RowsArgs a) {
-    grid_dependency_wait();
-    const int64_t step = (int64_t)gridDim.x * blockDim.x;
-    for (int64_t n = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; n < a.slots; n += step) {
-        const Slot s = slot_of<V>(a, n);
-        if (!s.in) continue;
-        float v[V], g[V], dy[V], o[V];
-        unpack<T, V>(ld_raw<T, V>(reinterpret_cast<const T*>(a.dy) + s.row * a.lddy + s.i), dy);
-        if constexpr (KEPT) {
-            const int64_t c = s.row * a.d + s.i, b = s.row * a.blocks + s.i / kBlock;
-            decode_as<T, V>(ld_raw<uint8_t, V>(a.qa + c), a.sa[b], a.e4m3, v);
-            if constexpr (GATED) decode_as<T, V>(ld_raw<uint8_t, V>(a.qb + c), a.sb[b], a.e4m3, g);
+template <typename T>
+__device__ __forceinline__ void any_restore(const RowsArgs& a, const Slot s[kAny], const uint8_t* q, const uint8_t* sc, float* v) {
+    uint8_t c[kAny];
+    uint32_t e[kAny];
+#pragma unroll
+    for (int k = 0; k < kAny; ++k) {
+        c[k] = 0;
+        e[k] = 0;
+        if (!s[k].in) continue;
+        c[k] = q[s[k].row * a.d + s[k].i];
+        e[k] = sc[s[k].row * a.blocks + s[k].i / kBlock];
+    }
+#pragma unroll
+    for (int k = 0; k < kAny; ++k) decode_as<T, 1>(c[k], e[k], a.e4m3, v + k);
+}
+// f and f' of kAny values.
+template <typename T, bool DERIV, bool FINITE>
+__device__ __forceinline__ void any_activate(int act, const float* v, float* f, float* df) {
+#pragma unroll
+    for (int k = 0; k < kAny; k += 2) {
+        if constexpr (sizeof(T) == 2) {
+            F2 x, y = 0;
+            if (act == kSilu) activate2<kSilu, DERIV, FINITE>(f2(v[k], v[k + 1]), x, y);
+            else activate2<kGelu, DERIV, FINITE>(f2(v[k], v[k + 1]), x, y);
+            const float2 fx = f2_parts(x), dx = f2_parts(y);
+            f[k] = fx.x; f[k + 1] = fx.y;
+            df[k] = dx.x; df[k + 1] = dx.y;
         } else {
-            unpack<T, V>(ld_raw<T, V>(reinterpret_cast<const T*>(a.a) + s.row * a.lda + s.i), v);
-            if constexpr (GATED) unpack<T, V>(ld_raw<T, V>(reinterpret_cast<const T*>(a.b) + s.row * a.ldb + s.i), g);
-        }
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            float f, df;
-            a.act == kSilu ? activate<kSilu>(v[i], f, df) : activate<kGelu>(v[i], f, df);
-            o[i] = dy[i] * df;
-            if constexpr (GATED) { o[i] *= g[i]; g[i] = dy[i] * f; }
+            for (int j = k; j < k + 2; ++j) {
+                if (act == kSilu) activate<kSilu>(v[j], f[j], df[j]);
+                else activate<kGelu>(v[j], f[j], df[j]);
+            }
         }
-        st_raw<T, V>(reinterpret_cast<T*>(a.da) + s.row * a.ldda + s.i, pack<T, V>(o));
-        if constexpr (GATED) st_raw<T, V>(reinterpret_cast<T*>(a.db) + s.row * a.lddb + s.i, pack<T, V>(g));
     }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256)
+quantize_any_kernel(RowsArgs a) {
+    grid_dependency_wait();
+    Slot s[kAny];
+    any_slots(a, s);
+    float v[kAny];
+    any_load<T>(a.a, a.lda, s, v);
+    any_keep(a, s, v, a.qa, a.sa);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256)
+dequantize_any_kernel(RowsArgs a) {
+    grid_dependency_wait();
+    Slot s[kAny];
+    any_slots(a, s);
+    float v[kAny];
+    any_restore<T>(a, s, a.qa, a.sa, v);
+    any_store<T>(a.y, a.ldy, s, v);
+}
+
+template <typename T, bool GATED>
+__global__ void __launch_bounds__(256)
+activation_any_kernel(RowsArgs a) {
+    grid_dependency_wait();
+    Slot s[kAny];
+    any_slots(a, s);
+    float v[kAny], g[kAny], o[kAny], df[kAny];
+    any_load<T>(a.a, a.lda, s, v);
+    if constexpr (GATED) any_load<T>(a.b, a.ldb, s, g);
+    any_activate<T, false, false>(a.act, v, o, df);
+    if constexpr (GATED) {
+#pragma unroll
+        for (int k = 0; k < kAny; ++k) o[k] *= g[k];
+    }
+    any_store<T>(a.y, a.ldy, s, o);
+    if (a.qa) any_keep(a, s, v, a.qa, a.sa);
+    if constexpr (GATED) { if (a.qb) any_keep(a, s, g, a.qb, a.sb); }
+}
+
+template <typename T, bool GATED, bool KEPT>
+__global__ void __launch_bounds__(256)
+activation_backward_any_kernel(RowsArgs a) {
+    grid_dependency_wait();
+    Slot s[kAny];
+    any_slots(a, s);
+    float dy[kAny], v[kAny], g[kAny], f[kAny], df[kAny];
+    any_load<T>(a.dy, a.lddy, s, dy);
+    if constexpr (KEPT) {
+        any_restore<T>(a, s, a.qa, a.sa, v);
+        if constexpr (GATED) any_restore<T>(a, s, a.qb, a.sb, g);
+    } else {
+        any_load<T>(a.a, a.lda, s, v);
+        if constexpr (GATED) any_load<T>(a.b, a.ldb, s, g);
+    }
+    any_activate<T, true, KEPT>(a.act, v, f, df);
+#pragma unroll
+    for (int k = 0; k < kAny; ++k) {
+        v[k] = dy[k] * df[k];
+        if constexpr (GATED) { v[k] *= g[k]; g[k] = dy[k] * f[k]; }
+    }
+    any_store<T>(a.da, a.ldda, s, v);
+    if constexpr (GATED) any_store<T>(a.db, a.lddb, s, g);
 }
 
 // ---- vectors ------------------------------------------------------------------------------------------
@@ -425,8 +469,8 @@ struct RowsCall {
 };
 
 template <typename K>
-static cudaError_t launch_rows(b200_stream_t st, K kernel, const RowsArgs& a) {
-    return launch_overlapped(kernel, balanced_grid((a.slots + 255) / 256, resident_blocks(kernel, 256, 0, st->dev)), 256u, 0, st->s, a);
+static cudaError_t launch_any(b200_stream_t st, K kernel, const RowsArgs& a) {
+    return launch_overlapped(kernel, (unsigned)((a.slots + 256 * kAny - 1) / (256 * kAny)), 256u, 0, st->s, a);
 }
 template <typename K>
 static cudaError_t launch_tiles(b200_stream_t st, K kernel, const RowsArgs& a) {
@@ -469,7 +513,7 @@ extern "C" int32_t b200_quantize(b200_stream_t st, const b200_tensor* Q, const b
     if (!v) return B200_OK;
     B200_CUDA(by_type(c.dtype, [&](auto t, auto w) {
         using T = decltype(t);
-        if (v == 1) return launch_rows(st, quantize_kernel<T, 1>, c.a);
+        if (v == 1) return launch_any(st, quantize_any_kernel<T>, c.a);
         return by_value<kInt8, kE4M3>(c.format(), [&](auto f) { return launch_tiles(st, quantize_vec_kernel<T, decltype(w)::value, decltype(f)::value>, c.a); });
     }));
     return finish(st, "b200_quantize");
@@ -486,7 +530,7 @@ extern "C" int32_t b200_dequantize(b200_stream_t st, const b200_tensor* X, const
     if (!v) return B200_OK;
     B200_CUDA(by_type(c.dtype, [&](auto t, auto w) {
         using T = decltype(t);
-        if (v == 1) return launch_rows(st, dequantize_kernel<T, 1>, c.a);
+        if (v == 1) return launch_any(st, dequantize_any_kernel<T>, c.a);
         return by_value<kInt8, kE4M3>(c.format(), [&](auto f) { return launch_tiles(st, dequantize_vec_kernel<T, decltype(w)::value, decltype(f)::value>, c.a); });
     }));
     return finish(st, "b200_dequantize");
@@ -513,7 +557,7 @@ extern "C" int32_t b200_activation(b200_stream_t st, int32_t act, const b200_ten
     B200_CUDA(by_type(c.dtype, [&](auto t, auto w) {
         using T = decltype(t);
         constexpr int V = decltype(w)::value;
-        if (v == 1) return B ? launch_rows(st, activation_kernel<T, 1, true>, c.a) : launch_rows(st, activation_kernel<T, 1, false>, c.a);
+        if (v == 1) return B ? launch_any(st, activation_any_kernel<T, true>, c.a) : launch_any(st, activation_any_kernel<T, false>, c.a);
         return by_value<kSilu, kGelu>(act, [&](auto f) {
             constexpr int ACT = decltype(f)::value;
             return by_value<kNoCodes, kInt8, kE4M3>(c.format(), [&](auto k) {
@@ -556,8 +600,8 @@ extern "C" int32_t b200_activation_backward(b200_stream_t st, int32_t act, const
         using T = decltype(t);
         constexpr int V = decltype(w)::value;
         if (v == 1) {
-            if (gated) return A ? launch_rows(st, activation_backward_kernel<T, 1, true, false>, c.a) : launch_rows(st, activation_backward_kernel<T, 1, true, true>, c.a);
-            return A ? launch_rows(st, activation_backward_kernel<T, 1, false, false>, c.a) : launch_rows(st, activation_backward_kernel<T, 1, false, true>, c.a);
+            if (gated) return A ? launch_any(st, activation_backward_any_kernel<T, true, false>, c.a) : launch_any(st, activation_backward_any_kernel<T, true, true>, c.a);
+            return A ? launch_any(st, activation_backward_any_kernel<T, false, false>, c.a) : launch_any(st, activation_backward_any_kernel<T, false, true>, c.a);
         }
         return by_value<kSilu, kGelu>(act, [&](auto f) {
             constexpr int ACT = decltype(f)::value;
