@@ -79,8 +79,8 @@ struct RowsArgs {
     const void *a, *b, *dy;
     void *y, *da, *db;
     uint8_t *qa, *sa, *qb, *sb;
-    int64_t lda, ldb, lddy, ldy, ldda, lddb, rows, d, blocks, slots;   // slots: rows * vectors per filled row
-    FastDiv per_row;                                                   // vectors per filled row
+    int64_t lda, ldb, lddy, ldy, ldda, lddb, rows, d, blocks, slots, total;   // slots: rows * vectors per filled row
+    FastDiv per_row;                                                   // vectors per filled row (dense rows of any width: d)
     int32_t e4m3, act, flat, small, wide;                              // wide: 32-byte accesses are aligned
 };
 
@@ -407,10 +407,234 @@ activation_backward_vec_kernel(RowsArgs a) {
     if constexpr (GATED) st_raw32(reinterpret_cast<T*>(a.db) + s.row * a.lddb + s.i, ob, a.wide);
 }
 
+// ---- dense rows of any width --------------------------------------------------------------------------
+// Rows without gaps are one long row for the loads and stores, so its vectors are aligned whatever d is; but
+// the blocks of 32 start anew with every row and begin and end inside vectors.  A vector of V <= 16 elements
+// meets three blocks at most (d >= 32: only a row's last block is shorter than 32), whose scale bytes are
+// neighbours.  A block's largest magnitude is collected in shared memory over the tile's threads; of the
+// blocks that reach over the tile's ends the missing elements are read as well (31 at most either side).
+struct Cuts {
+    int64_t f, scale;          // first element, its block
+    int b1, b2, n;             // elements of the first block, of the first two; elements in the array
+    bool opens;                // the first block starts here
+};
+template <int V>
+__device__ __forceinline__ Cuts cuts_of(const RowsArgs& a, int64_t f) {
+    Cuts c;
+    c.f = f;
+    const int64_t left = a.total - f, d = a.per_row.d;
+    c.n = left <= 0 ? 0 : left < V ? (int)left : V;
+    const int64_t row = a.small ? (int64_t)a.per_row.div((uint32_t)f) : f / d;
+    int64_t i = f - row * d;
+    c.scale = row * a.blocks + i / kBlock;
+    c.opens = i % kBlock == 0;
+    c.b1 = (int)min((int64_t)kBlock - i % kBlock, d - i);
+    i += c.b1;
+    if (i == d) i = 0;
+    c.b2 = c.b1 + (int)min((int64_t)kBlock, d - i);
+    return c;
+}
+template <typename T, int V>
+__device__ __forceinline__ RawVec<T, V> cut_load(const void* p, const Cuts& c, bool wide) {
+    const T* at = reinterpret_cast<const T*>(p) + c.f;
+    if (c.n == V) return ld_raw32(at, wide);
+    RawVec<T, V> r{};
+#pragma unroll
+    for (int j = 0; j < V; ++j) if (j < c.n) reinterpret_cast<T*>(&r)[j] = at[j];
+    return r;
+}
+template <typename T, int V>
+__device__ __forceinline__ void cut_store(void* p, const Cuts& c, const RawVec<T, V>& r, bool wide) {
+    T* at = reinterpret_cast<T*>(p) + c.f;
+    if (c.n == V) { st_raw32(at, r, wide); return; }
+#pragma unroll
+    for (int j = 0; j < V; ++j) if (j < c.n) at[j] = reinterpret_cast<const T*>(&r)[j];
+}
+template <typename X>
+__device__ __forceinline__ X cut_pick(const Cuts& c, int j, X x0, X x1, X x2) { return j < c.b1 ? x0 : j < c.b2 ? x1 : x2; }
+
+// Codes and scale bytes of the tile's rows; `most`: room for the magnitudes of the tile's blocks.
+constexpr int kCutBlocks = 288;          // of 256 vectors of 16 elements: 2 blocks per 33 elements, and the ends
+template <typename T, int V, int F>
+__device__ __forceinline__ void cut_keep(const RowsArgs& a, const Cuts& c, const RawVec<T, V>& r, const T* p, uint8_t* q, uint8_t* sc, uint32_t* most) {
+    const int64_t f0 = (int64_t)blockIdx.x * 256 * V;
+    const Cuts lo = cuts_of<V>(a, f0);
+    for (int i = threadIdx.x; i < kCutBlocks; i += 256) most[i] = 0;
+    __syncthreads();
+    F2 v[V / 2];
+    unpack2<T, V>(r, v);
+    uint32_t m[3] = {0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < V; ++j) {                             // elements past the array are zeros
+        const float2 x = f2_parts(v[j / 2]);
+        const uint32_t bits = __float_as_uint(j & 1 ? x.y : x.x) & 0x7fffffffu;
+        if (j < c.b1) m[0] = max(m[0], bits);
+        else if (j < c.b2) m[1] = max(m[1], bits);
+        else m[2] = max(m[2], bits);
+    }
+    const int at = (int)(c.scale - lo.scale);
+    if (c.n > 0) {
+        atomicMax(most + at, m[0]);
+        if (c.b1 < c.n) atomicMax(most + at + 1, m[1]);
+        if (c.b2 < c.n) atomicMax(most + at + 2, m[2]);
+    }
+    if (threadIdx.x < 32) {                                   // before the tile
+        const int64_t row = lo.scale / a.blocks;
+        const int64_t start = row * (int64_t)a.per_row.d + (lo.scale - row * a.blocks) * kBlock;
+        if (start + threadIdx.x < f0) atomicMax(most, __float_as_uint(Elem<T>::get(p[start + threadIdx.x])) & 0x7fffffffu);
+    } else if (threadIdx.x < 64) {                            // behind it
+        const int64_t end = f0 + 256 * V;
+        if (end < a.total) {
+            const Cuts hi = cuts_of<V>(a, end);
+            const int lane = threadIdx.x - 32;
+            if (!hi.opens && lane < hi.b1 && end + lane < a.total)
+                atomicMax(most + (hi.scale - lo.scale), __float_as_uint(Elem<T>::get(p[end + lane])) & 0x7fffffffu);
+        }
+    }
+    __syncthreads();
+    if (c.n == 0) return;
+    uint32_t e[3];
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+        e[k] = scale_byte(__uint_as_float(most[at + k]), F == kE4M3);
+        const int first = k == 0 ? 0 : k == 1 ? c.b1 : c.b2;
+        if (first < c.n && (k > 0 || c.opens)) sc[c.scale + k] = (uint8_t)e[k];
+    }
+    RawVec<uint8_t, V> codes{};
+    if (max(e[0], max(e[1], e[2])) < 255u) {
+        const float i0 = inverse_scale(e[0]), i1 = inverse_scale(e[1]), i2 = inverse_scale(e[2]);
+        uint32_t* w = reinterpret_cast<uint32_t*>(&codes);
+#pragma unroll
+        for (int j = 0; j < V; j += 4) {
+            const F2 p0 = f2(cut_pick(c, j, i0, i1, i2), cut_pick(c, j + 1, i0, i1, i2)), p1 = f2(cut_pick(c, j + 2, i0, i1, i2), cut_pick(c, j + 3, i0, i1, i2));
+            if constexpr (F == kE4M3) {
+                const float2 x = f2_parts(f2_mul(v[j / 2], p0)), y = f2_parts(f2_mul(v[j / 2 + 1], p1));
+                w[j / 4] = e4m3_pair(x.x, x.y) | e4m3_pair(y.x, y.y) << 16;
+            } else {
+                const F2 magic = f2(12582912.f);
+                const float2 x = f2_parts(f2_fma(v[j / 2], p0, magic)), y = f2_parts(f2_fma(v[j / 2 + 1], p1, magic));
+                w[j / 4] = __byte_perm(__byte_perm(__float_as_uint(x.x), __float_as_uint(x.y), 0x0040), __byte_perm(__float_as_uint(y.x), __float_as_uint(y.y), 0x0040), 0x5410);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const float2 x = f2_parts(v[j / 2]);
+            const float one = j & 1 ? x.y : x.x;
+            reinterpret_cast<uint8_t*>(&codes)[j] = encode<1>(&one, cut_pick(c, j, e[0], e[1], e[2]), F == kE4M3);
+        }
+    }
+    uint8_t* to = q + c.f;
+    if (c.n == V) {
+        st_raw<uint8_t, V>(to, codes);
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) if (j < c.n) to[j] = reinterpret_cast<const uint8_t*>(&codes)[j];
+    }
+}
+template <typename T, int V, int F>
+__device__ __forceinline__ void cut_restore(const Cuts& c, const uint8_t* q, const uint8_t* sc, F2* v) {
+    RawVec<uint8_t, V> r{};
+    const uint8_t* at = q + c.f;
+    if (c.n == V) {
+        r = ld_raw<uint8_t, V>(at);
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) if (j < c.n) reinterpret_cast<uint8_t*>(&r)[j] = at[j];
+    }
+    const uint32_t e0 = sc[c.scale], e1 = c.b1 < c.n ? sc[c.scale + 1] : e0, e2 = c.b2 < c.n ? sc[c.scale + 2] : e0;
+    if (plain_scale<T>(max(e0, max(e1, e2)))) {
+        const float s0 = scale_value(e0), s1 = scale_value(e1), s2 = scale_value(e2);
+        decode2<V>(r, 127u, F == kE4M3, v);                   // at scale one
+#pragma unroll
+        for (int j = 0; j < V; j += 2) v[j / 2] = f2_mul(v[j / 2], f2(cut_pick(c, j, s0, s1, s2), cut_pick(c, j + 1, s0, s1, s2)));
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; j += 2) {
+            float x[2];
+            decode_as<T, 1>(reinterpret_cast<const uint8_t*>(&r)[j], cut_pick(c, j, e0, e1, e2), F == kE4M3, x);
+            decode_as<T, 1>(reinterpret_cast<const uint8_t*>(&r)[j + 1], cut_pick(c, j + 1, e0, e1, e2), F == kE4M3, x + 1);
+            v[j / 2] = f2(x[0], x[1]);
+        }
+    }
+}
+
+template <typename T, int V, int F>
+__global__ void __launch_bounds__(256)
+quantize_cut_kernel(RowsArgs a) {
+    __shared__ uint32_t most[kCutBlocks];
+    grid_dependency_wait();
+    const Cuts c = cuts_of<V>(a, ((int64_t)blockIdx.x * 256 + threadIdx.x) * V);
+    cut_keep<T, V, F>(a, c, cut_load<T, V>(a.a, c, a.wide), reinterpret_cast<const T*>(a.a), a.qa, a.sa, most);
+}
+template <typename T, int V, int F>
+__global__ void __launch_bounds__(256)
+dequantize_cut_kernel(RowsArgs a) {
+    grid_dependency_wait();
+    const Cuts c = cuts_of<V>(a, ((int64_t)blockIdx.x * 256 + threadIdx.x) * V);
+    if (c.n == 0) return;
+    F2 v[V / 2];
+    cut_restore<T, V, F>(c, a.qa, a.sa, v);
+    cut_store<T, V>(a.y, c, pack2<T, V>(v), a.wide);
+}
+template <typename T, int V, int ACT, bool GATED, int F>
+__global__ void __launch_bounds__(256)
+activation_cut_kernel(RowsArgs a) {
+    __shared__ uint32_t most[GATED ? 2 : 1][F == kNoCodes ? 1 : kCutBlocks];
+    grid_dependency_wait();
+    const Cuts c = cuts_of<V>(a, ((int64_t)blockIdx.x * 256 + threadIdx.x) * V);
+    const RawVec<T, V> ra = cut_load<T, V>(a.a, c, a.wide);
+    RawVec<T, V> rb{};
+    if constexpr (GATED) rb = cut_load<T, V>(a.b, c, a.wide);
+    F2 v[V / 2], g[V / 2];
+    unpack2<T, V>(ra, v);
+    if constexpr (GATED) unpack2<T, V>(rb, g);
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+        F2 f, df;
+        activate_pair<ACT, sizeof(T) == 2, false, false>(v[i], f, df);
+        v[i] = GATED ? f2_mul(f, g[i]) : f;
+    }
+    cut_store<T, V>(a.y, c, pack2<T, V>(v), a.wide);
+    if constexpr (F != kNoCodes) {
+        if (a.qa) cut_keep<T, V, F>(a, c, ra, reinterpret_cast<const T*>(a.a), a.qa, a.sa, most[0]);
+        if constexpr (GATED) { if (a.qb) cut_keep<T, V, F>(a, c, rb, reinterpret_cast<const T*>(a.b), a.qb, a.sb, most[1]); }
+    }
+}
+template <typename T, int V, int ACT, bool GATED, int F>
+__global__ void __launch_bounds__(256)
+activation_backward_cut_kernel(RowsArgs a) {
+    grid_dependency_wait();
+    const Cuts c = cuts_of<V>(a, ((int64_t)blockIdx.x * 256 + threadIdx.x) * V);
+    if (c.n == 0) return;
+    const RawVec<T, V> rd = cut_load<T, V>(a.dy, c, a.wide);
+    F2 dy[V / 2], v[V / 2], g[V / 2];
+    if constexpr (F != kNoCodes) {
+        cut_restore<T, V, F>(c, a.qa, a.sa, v);
+        if constexpr (GATED) cut_restore<T, V, F>(c, a.qb, a.sb, g);
+    } else {
+        unpack2<T, V>(cut_load<T, V>(a.a, c, a.wide), v);
+        if constexpr (GATED) unpack2<T, V>(cut_load<T, V>(a.b, c, a.wide), g);
+    }
+    unpack2<T, V>(rd, dy);
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+        F2 f, df;
+        activate_pair<ACT, sizeof(T) == 2, true, F != kNoCodes>(v[i], f, df);
+        v[i] = f2_mul(dy[i], df);
+        if constexpr (GATED) { v[i] = f2_mul(v[i], g[i]); g[i] = f2_mul(dy[i], f); }
+    }
+    cut_store<T, V>(a.da, c, pack2<T, V>(v), a.wide);
+    if constexpr (GATED) cut_store<T, V>(a.db, c, pack2<T, V>(g), a.wide);
+}
+
 // ---- host ---------------------------------------------------------------------------------------
+enum { kCut = -1 };
+
 struct RowsCall {
     RowsArgs a{};
-    bool dense = true, aligned = true, aligned32 = true;
+    bool dense = true, aligned = true, aligned32 = true;       // of every row; below: of the arrays' beginnings
+    bool base = true, base32 = true, apart = true;             // apart: nothing is written over what a neighbour reads
     int32_t dtype = -1;
 
     int32_t in(const b200_tensor* t, const b200_tensor* like, const char* name, const void** p, int64_t* ld) {
@@ -433,6 +657,8 @@ struct RowsCall {
         dense = dense && (v.rows <= 1 || v.ld == v.d);
         aligned = aligned && rows_aligned(v, 16);
         aligned32 = aligned32 && rows_aligned(v, 32);
+        base = base && reinterpret_cast<uintptr_t>(v.p) % 16 == 0;
+        base32 = base32 && reinterpret_cast<uintptr_t>(v.p) % 32 == 0;
         *p = v.p;
         *ld = v.ld;
         return B200_OK;
@@ -444,18 +670,28 @@ struct RowsCall {
         const int32_t e4m3 = Q->dtype == B200_U8;
         if (!first && e4m3 != a.e4m3) return fail(B200_INVALID_ARG, "%s: one call keeps both operands in one format", name);
         a.e4m3 = e4m3;
-        aligned = aligned && reinterpret_cast<uintptr_t>(Q->ptr) % 16 == 0;
+        base = base && reinterpret_cast<uintptr_t>(Q->ptr) % 16 == 0;
+        aligned = aligned && base;
         *q = (uint8_t*)Q->ptr;
         *s = (uint8_t*)S->ptr;
         return B200_OK;
     }
     int format() const { return !(a.qa || a.qb) ? (int)kNoCodes : a.e4m3 ? (int)kE4M3 : (int)kInt8; }
-    // Vector width, and the slots for it; 0: nothing to do.
+    // Vector width, and the slots for it (kCut: dense rows of any width); 0: nothing to do.
     int plan() {
         if (a.rows == 0 || a.d == 0) return 0;
         const int full = dtype == B200_F32 ? 8 : 16;
         const int v = aligned && a.d % full == 0 ? full : 1;
         a.wide = aligned32;
+        a.total = a.rows * a.d;
+        if (v == 1 && dense && base && apart && a.d >= kBlock && a.d <= 0x7fffffff) {
+            a.wide = base32;
+            a.blocks = row_blocks(a.d);
+            a.slots = (a.total + full - 1) / full;
+            a.small = a.total < (int64_t)0x7fff0000;
+            a.per_row = FastDiv((uint32_t)a.d);
+            return kCut;
+        }
         a.blocks = row_blocks(a.d);
         a.flat = dense && a.d % kBlock == 0;
         if (a.flat) { a.d *= a.rows; a.blocks *= a.rows; a.rows = 1; }
@@ -514,7 +750,10 @@ extern "C" int32_t b200_quantize(b200_stream_t st, const b200_tensor* Q, const b
     B200_CUDA(by_type(c.dtype, [&](auto t, auto w) {
         using T = decltype(t);
         if (v == 1) return launch_any(st, quantize_any_kernel<T>, c.a);
-        return by_value<kInt8, kE4M3>(c.format(), [&](auto f) { return launch_tiles(st, quantize_vec_kernel<T, decltype(w)::value, decltype(f)::value>, c.a); });
+        return by_value<kInt8, kE4M3>(c.format(), [&](auto f) {
+            constexpr int V = decltype(w)::value, F = decltype(f)::value;
+            return v == kCut ? launch_tiles(st, quantize_cut_kernel<T, V, F>, c.a) : launch_tiles(st, quantize_vec_kernel<T, V, F>, c.a);
+        });
     }));
     return finish(st, "b200_quantize");
 }
@@ -531,7 +770,10 @@ extern "C" int32_t b200_dequantize(b200_stream_t st, const b200_tensor* X, const
     B200_CUDA(by_type(c.dtype, [&](auto t, auto w) {
         using T = decltype(t);
         if (v == 1) return launch_any(st, dequantize_any_kernel<T>, c.a);
-        return by_value<kInt8, kE4M3>(c.format(), [&](auto f) { return launch_tiles(st, dequantize_vec_kernel<T, decltype(w)::value, decltype(f)::value>, c.a); });
+        return by_value<kInt8, kE4M3>(c.format(), [&](auto f) {
+            constexpr int V = decltype(w)::value, F = decltype(f)::value;
+            return v == kCut ? launch_tiles(st, dequantize_cut_kernel<T, V, F>, c.a) : launch_tiles(st, dequantize_vec_kernel<T, V, F>, c.a);
+        });
     }));
     return finish(st, "b200_dequantize");
 }
@@ -549,6 +791,7 @@ extern "C" int32_t b200_activation(b200_stream_t st, int32_t act, const b200_ten
     B200_TRY(c.out(Y, A, "activation destination", &c.a.y, &c.a.ldy));
     if (QA) B200_TRY(c.codes(QA, SA, A, "activation checkpoint", &c.a.qa, &c.a.sa, true));
     if (QB) B200_TRY(c.codes(QB, SB, A, "gate checkpoint", &c.a.qb, &c.a.sb, !QA));
+    c.apart = !(QA || QB) || (c.a.y != c.a.a && c.a.y != c.a.b);
     const int v = c.plan();
     if (v) B200_TRY(row_limit(c));
     B200_TRY(enter(st));
@@ -562,6 +805,7 @@ extern "C" int32_t b200_activation(b200_stream_t st, int32_t act, const b200_ten
             constexpr int ACT = decltype(f)::value;
             return by_value<kNoCodes, kInt8, kE4M3>(c.format(), [&](auto k) {
                 constexpr int F = decltype(k)::value;
+                if (v == kCut) return B ? launch_tiles(st, activation_cut_kernel<T, V, ACT, true, F>, c.a) : launch_tiles(st, activation_cut_kernel<T, V, ACT, false, F>, c.a);
                 return B ? launch_tiles(st, activation_vec_kernel<T, V, ACT, true, F>, c.a) : launch_tiles(st, activation_vec_kernel<T, V, ACT, false, F>, c.a);
             });
         });
@@ -607,6 +851,9 @@ extern "C" int32_t b200_activation_backward(b200_stream_t st, int32_t act, const
             constexpr int ACT = decltype(f)::value;
             return by_value<kNoCodes, kInt8, kE4M3>(c.format(), [&](auto k) {
                 constexpr int F = decltype(k)::value;
+                if (v == kCut)
+                    return gated ? launch_tiles(st, activation_backward_cut_kernel<T, V, ACT, true, F>, c.a)
+                                 : launch_tiles(st, activation_backward_cut_kernel<T, V, ACT, false, F>, c.a);
                 return gated ? launch_tiles(st, activation_backward_vec_kernel<T, V, ACT, true, F>, c.a)
                              : launch_tiles(st, activation_backward_vec_kernel<T, V, ACT, false, F>, c.a);
             });

@@ -181,3 +181,38 @@ def test_layouts_and_aliases(gpu):
         assert gpu.activation("silu", x).dims == dims and gpu.dequantize(gpu.quantize(x)).dims == dims
     x = gpu.ROCArray.from_host(rng.standard_normal((33, 4, 5)).astype(np.float32))
     assert gpu.dequantize(gpu.quantize(x, "e4m3")).dims == (33, 4, 5)
+
+
+@pytest.mark.parametrize("d,n", [(33, 1000), (46, 333), (63, 700), (1023, 50), (40, 513), (2049, 9), (33, 8), (35, 117)])
+def test_blocks_across_vectors(gpu, d, n):
+    """Dense rows of odd widths: blocks begin and end inside vectors and across the tiles of a launch; codes,
+    scale bytes and what comes back stay those of the rows, for every type, and so do both passes."""
+    for name, t in ref.TYPES.items():
+        rng = np.random.default_rng(d)
+        x = values(rng, d, n, t, True)
+        x[:, ::3] = values(rng, d, n, t, False)[:, ::3]
+        if n > 5:
+            x[d // 2, 5], x[d - 1, 3] = np.nan, np.inf
+        X, G = gpu.ROCArray.from_host(x), gpu.ROCArray.from_host(np.roll(x, 1, axis=1))
+        for form in ("int8", "e4m3"):
+            codes, scales = Guarded(gpu, np.int8 if form == "int8" else np.uint8, (d, n)), Guarded(gpu, np.uint8, (-(-d // 32), n))
+            q = gpu.Quantized8.wrap(codes.array, scales.array)
+            gpu.quantize_(q, X)
+            c, e = ref.quantize(x.astype(np.float64), form)
+            assert np.array_equal(scales.array.to_host(), e), (name, form)
+            assert np.array_equal(ref.restore(codes.array.to_host(), e), ref.restore(c, e), equal_nan=True), (name, form)
+            y = Guarded(gpu, t, (d, n))
+            gpu.dequantize_(y.array, q)
+            ref.within(y.array.to_host(), ref.saturated(ref.restore(c, e), t), 0.0, (name, form))
+            y.check(); codes.check(); scales.check()
+            qa, qb = gpu.Quantized8((d, n), form), gpu.Quantized8((d, n), form)
+            Y = Guarded(gpu, t, (d, n))
+            gpu.activation_("silu", Y.array, X, G, checkpoint=qa, gate_checkpoint=qb)
+            Y.check()
+            assert bits_equal(qa.codes.to_host(), q.codes.to_host()) and bits_equal(qa.scales.to_host(), e)
+            assert np.array_equal(qb.scales.to_host(), np.roll(e, 1, axis=1))
+            # in place: the same results by the kernel that reads nothing of its neighbours
+            Z, qz, qy = X.copy(), gpu.Quantized8((d, n), form), gpu.Quantized8((d, n), form)
+            gpu.activation_("silu", Z, Z, G, checkpoint=qz, gate_checkpoint=qy)
+            assert np.array_equal(Z.to_host(), Y.array.to_host(), equal_nan=True) and bits_equal(qz.codes.to_host(), qa.codes.to_host())
+            assert bits_equal(qy.scales.to_host(), qb.scales.to_host())
