@@ -8,7 +8,6 @@ from __future__ import annotations
 
 from ._lib import check, lib
 from .array import ROCArray, on_stream
-from .normalization import _ptr
 from .quantization import Quantized8, rows_back, rows_in, rows_out
 from .runtime import Stream, current_stream
 
@@ -37,9 +36,9 @@ def activation_(f: str, Y: ROCArray, A: ROCArray, gate: ROCArray | None = None, 
     Ar, Br, Yr = rows_in(A, 1, st), rows_in(gate, 1, st), rows_out(Y, 1, st)
     qa, sa = (None, None) if checkpoint is None else (checkpoint.codes, checkpoint.scales)
     qb, sb = (None, None) if gate_checkpoint is None else (gate_checkpoint.codes, gate_checkpoint.scales)
-    on_stream(st, Yr, Ar, Br, qa, sa, qb, sb)
-    check(lib.b200_activation(st.handle, act, Yr._ref(), Ar._ref(), _ptr(Br), _ptr(qa), _ptr(sa), _ptr(qb), _ptr(sb)))
-    rows_back(Y, Yr, st)
+    check(lib.b200_activation(st.handle, act, *on_stream(st, Yr, Ar, Br, qa, sa, qb, sb)))
+    if Yr is not Y:
+        rows_back(Y, Yr, st)
     return Y
 
 
@@ -69,9 +68,7 @@ def activation_backward_(f: str, dA: ROCArray, dY: ROCArray, A: "ROCArray | Quan
             qb, sb = gate.codes, gate.scales
     else:
         a, b = rows_in(A, 1, st), rows_in(gate, 1, st)
-    on_stream(st, dAr, dBr, dYr, a, b, qa, sa, qb, sb)
-    check(lib.b200_activation_backward(st.handle, act, dAr._ref(), _ptr(dBr), dYr._ref(), _ptr(a), _ptr(b),
-                                       _ptr(qa), _ptr(sa), _ptr(qb), _ptr(sb)))
+    check(lib.b200_activation_backward(st.handle, act, *on_stream(st, dAr, dBr, dYr, a, b, qa, sa, qb, sb)))
     rows_back(dA, dAr, st)
     rows_back(dgate, dBr, st)
     return dA

@@ -98,14 +98,24 @@ def with_managed(stream: Stream, *arrays) -> Stream:
     return stream
 
 
-def on_stream(stream: Stream, *arrays) -> Stream:
-    """:func:`with_managed` for operators that refuse arrays of another device than the stream's."""
+def on_stream(stream: Stream, *arrays) -> list:
+    """:func:`with_managed` for operators that refuse arrays of another device than the stream's; returns
+    references to the arrays' descriptors, in their order (``None`` stays).  One walk over the arrays:
+    a call on few elements is as long as its host side."""
+    refs = []
     for a in arrays:
-        if a is not None:
-            if a.buf.device != stream.device:
-                raise ValueError(f"an array of device {a.buf.device} cannot be used on a stream of device {stream.device}")
-            a.buf.take_ownership(stream)
-    return stream
+        if a is None:
+            refs.append(None)
+            continue
+        b = a.buf
+        if b.stream is stream:
+            b.dirty = True
+        else:
+            if b.device != stream.device:
+                raise ValueError(f"an array of device {b.device} cannot be used on a stream of device {stream.device}")
+            b.take_ownership(stream)
+        refs.append(a._ref())
+    return refs
 
 
 class ROCArray:

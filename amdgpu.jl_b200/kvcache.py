@@ -53,7 +53,7 @@ def quantized_cache(head_dim: int, heads: int, page_size: int, pages: int, forma
 
 
 def _neighbours(A: ROCArray, st: Stream) -> ROCArray:
-    return A if A.strides[:1] == (1,) or A.dims[:1] == (1,) else A.copy(st)
+    return A if A._strides is None or A._strides[:1] == (1,) or A.dims[:1] == (1,) else A.copy(st)
 
 
 def cache_write_(cache: QuantizedCache, K: ROCArray, V: ROCArray, slots: ROCArray, *, rotary: RotaryPlan | None = None,
@@ -68,13 +68,8 @@ def cache_write_(cache: QuantizedCache, K: ROCArray, V: ROCArray, slots: ROCArra
     K, V = _neighbours(K, st), _neighbours(V, st)
     kq, ks, vq, vs = cache._arrays()
     table = None if rotary is None else rotary.table
-    on_stream(st, kq, ks, vq, vs, K, V, slots, positions, table)
-    if rotary is None:
-        status = lib.b200_cache_write(st.handle, kq._ref(), ks._ref(), vq._ref(), vs._ref(), K._ref(), V._ref(), slots._ref(), None, None, 0, 1.0)
-    else:
-        status = lib.b200_cache_write(st.handle, kq._ref(), ks._ref(), vq._ref(), vs._ref(), K._ref(), V._ref(), slots._ref(),
-                                      positions._ref(), table._ref(), rotary._layout, rotary.factor)
-    check(status)
+    layout, factor = (0, 1.0) if rotary is None else (rotary._layout, rotary.factor)
+    check(lib.b200_cache_write(st.handle, *on_stream(st, kq, ks, vq, vs, K, V, slots, positions, table), layout, factor))
     return cache
 
 
@@ -86,6 +81,5 @@ def cache_read_(K: ROCArray, V: ROCArray, cache: QuantizedCache, pages: ROCArray
     as an error at the next synchronisation; what is in range is read."""
     st = stream or current_stream()
     kq, ks, vq, vs = cache._arrays()
-    on_stream(st, K, V, kq, ks, vq, vs, pages, lengths)
-    check(lib.b200_cache_read(st.handle, K._ref(), V._ref(), kq._ref(), ks._ref(), vq._ref(), vs._ref(), pages._ref(), lengths._ref()))
+    check(lib.b200_cache_read(st.handle, *on_stream(st, K, V, kq, ks, vq, vs, pages, lengths)))
     return K, V

@@ -18,19 +18,17 @@ from .runtime import Stream, current_stream
 def _lead(X, lead, *params) -> int:
     for p in params:
         if p is not None:
-            if lead is not None and lead != p.ndim:
+            n = len(p.dims)
+            if lead is not None and lead != n:
                 raise ValueError("layernorm: `lead` and the parameters differ in dimensions")
-            lead = p.ndim
-            if p.dims != X.dims[:lead]:
-                raise ValueError(f"layernorm: parameters of size {p.dims} for rows of size {X.dims[:lead]}")
-    lead = 1 if lead is None else int(lead)
+            lead = n
+            if p.dims != X.dims[:n]:
+                raise ValueError(f"layernorm: parameters of size {p.dims} for rows of size {X.dims[:n]}")
+    if lead is None:
+        lead = 1
     if not 1 <= lead <= len(X.dims):
         raise ValueError("layernorm: `lead` counts the normalised dimensions, 1 to ndims")
     return lead
-
-
-def _ptr(a):
-    return None if a is None else a._ref()
 
 
 def layernorm_(Y: ROCArray, X: ROCArray, gamma: ROCArray | None = None, beta: ROCArray | None = None, *, eps: float = 1e-5,
@@ -49,9 +47,10 @@ def layernorm_(Y: ROCArray, X: ROCArray, gamma: ROCArray | None = None, beta: RO
     Xr = rows_in(X, lead, st)
     Yr = Xr if Y is X and Xr is X else rows_out(Y, lead, st)
     q, s = (None, None) if checkpoint is None else (checkpoint.codes, checkpoint.scales)
-    on_stream(st, Yr, Xr, gamma, beta, mean, rstd, q, s)
-    check(lib.b200_layernorm(st.handle, Yr._ref(), Xr._ref(), lead, _ptr(gamma), _ptr(beta), eps, _ptr(mean), _ptr(rstd), _ptr(q), _ptr(s)))
-    rows_back(Y, Yr, st)
+    y, x, g, b, *kept = on_stream(st, Yr, Xr, gamma, beta, mean, rstd, q, s)
+    check(lib.b200_layernorm(st.handle, y, x, lead, g, b, eps, *kept))
+    if Yr is not Y:
+        rows_back(Y, Yr, st)
     return Y
 
 
@@ -79,10 +78,10 @@ def layernorm_backward_(dX: ROCArray | None, dY: ROCArray, X: "ROCArray | Quanti
     dYr, Xr = rows_in(dY, lead, st), X if kept else rows_in(X, lead, st)
     dXr = rows_out(dX, lead, st)
     x, q, s = (None, X.codes, X.scales) if kept else (Xr, None, None)
-    on_stream(st, dXr, dYr, x, q, s, gamma, mean, rstd, dgamma, dbeta)
-    check(lib.b200_layernorm_backward(st.handle, _ptr(dXr), _ptr(dgamma), _ptr(dbeta), dYr._ref(), lead, _ptr(x), _ptr(q), _ptr(s),
-                                      _ptr(gamma), _ptr(mean), rstd._ref()))
-    rows_back(dX, dXr, st)
+    dx, dg, db, dy, *rest = on_stream(st, dXr, dgamma, dbeta, dYr, x, q, s, gamma, mean, rstd)
+    check(lib.b200_layernorm_backward(st.handle, dx, dg, db, dy, lead, *rest))
+    if dXr is not dX:
+        rows_back(dX, dXr, st)
     return dX
 
 

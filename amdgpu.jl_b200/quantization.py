@@ -97,8 +97,7 @@ def quantize_(q: Quantized8, X: ROCArray, stream: Stream | None = None) -> Quant
     """Rows of `X` (Float16, BFloat16 or Float32) to 8 bits."""
     st = stream or current_stream()
     Xr = rows_in(X, 1, st)
-    on_stream(st, q.codes, q.scales, Xr)
-    check(lib.b200_quantize(st.handle, q.codes._ref(), q.scales._ref(), Xr._ref()))
+    check(lib.b200_quantize(st.handle, *on_stream(st, q.codes, q.scales, Xr)))
     return q
 
 
@@ -111,8 +110,7 @@ def dequantize_(X: ROCArray, q: Quantized8, stream: Stream | None = None) -> ROC
     """What the codes stand for, rounded to `X`'s type; values past its range become its largest."""
     st = stream or current_stream()
     Xr = rows_out(X, 1, st)
-    on_stream(st, Xr, q.codes, q.scales)
-    check(lib.b200_dequantize(st.handle, Xr._ref(), q.codes._ref(), q.scales._ref()))
+    check(lib.b200_dequantize(st.handle, *on_stream(st, Xr, q.codes, q.scales)))
     rows_back(X, Xr, st)
     return X
 

@@ -84,7 +84,6 @@ def rotary_(Y: ROCArray, X: ROCArray, positions: ROCArray, plan: RotaryPlan, *, 
     if Y.dims != X.dims or Y.dtype != X.dtype:
         raise ValueError("rotary: source and destination must have the same size and element type")
     st = stream or current_stream()
-    Xr = X if X.strides[:1] == (1,) or X.dims[:1] == (1,) else X.copy(st)
-    on_stream(st, Y, Xr, positions, plan.table)
-    check(lib.b200_rotary(st.handle, Y._ref(), Xr._ref(), positions._ref(), plan.table._ref(), plan._layout, plan.factor, 1 if adjoint else 0))
+    Xr = X if X._strides is None or X._strides[:1] == (1,) or X.dims[:1] == (1,) else X.copy(st)
+    check(lib.b200_rotary(st.handle, *on_stream(st, Y, Xr, positions, plan.table), plan._layout, plan.factor, 1 if adjoint else 0))
     return Y
