@@ -128,6 +128,7 @@ __device__ __forceinline__ void ring_copy(void* dst, const void* src) {
 }
 template <typename T, int V, int NV>
 __device__ __forceinline__ void load_params2(const NormArgs& a, const void* p, int t, int nvec, float missing, F2* out) {
+    const bool aligned = (reinterpret_cast<uintptr_t>(p) & 15) == 0;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
         const int vi = t + k * a.group;
@@ -138,14 +139,19 @@ __device__ __forceinline__ void load_params2(const NormArgs& a, const void* p, i
 #pragma unroll
             for (int i = 0; i < V / 4; ++i) {
                 const float* f = reinterpret_cast<const float*>(p) + (int64_t)vi * V + 4 * i;
-                out[k * V / 2 + 2 * i] = f2(f[0], f[1]);
-                out[k * V / 2 + 2 * i + 1] = f2(f[2], f[3]);
+                float4 q;
+                if (aligned) q = *reinterpret_cast<const float4*>(f);
+                else q = make_float4(f[0], f[1], f[2], f[3]);
+                out[k * V / 2 + 2 * i] = f2(q.x, q.y);
+                out[k * V / 2 + 2 * i + 1] = f2(q.z, q.w);
             }
         } else {
+            const T* f = reinterpret_cast<const T*>(p) + (int64_t)vi * V;
+            if (aligned) {
+                unpack2<T, V>(ld_raw_cached<T, V>(f), out + k * V / 2);
+            } else {
 #pragma unroll
-            for (int i = 0; i < V / 2; ++i) {
-                const T* f = reinterpret_cast<const T*>(p) + (int64_t)vi * V + 2 * i;
-                out[k * V / 2 + i] = f2(Elem<T>::get(f[0]), Elem<T>::get(f[1]));
+                for (int i = 0; i < V / 2; ++i) out[k * V / 2 + i] = f2(Elem<T>::get(f[2 * i]), Elem<T>::get(f[2 * i + 1]));
             }
         }
     }
@@ -955,7 +961,8 @@ struct NormLaunch {
 template <typename T, int E, int STAGES, int THREADS>
 static cudaError_t forward_ring(b200_stream_t st, const NormArgs& a) {
     NormLaunch l{st, a};
-    const int per = a.group >= 256 ? 1 : 256 / a.group;
+    int per = a.group >= 256 ? 1 : 256 / a.group;
+    while (per > 1 && a.rows < (int64_t)per * sm_count(st->dev) && (per / 2) * a.group >= 32) per /= 2;      // few rows: an SM each
     const size_t bytes = (size_t)STAGES * (E * sizeof(T)) * THREADS;
     auto run = [&](auto kernel) { const cudaError_t e = l.plan(kernel, per, bytes); return e == cudaSuccess ? l.go(kernel) : e; };
     if (!a.q) return run(norm_forward_ring_kernel<T, E, STAGES, THREADS, kAsIs>);
