@@ -506,18 +506,22 @@ template <int W>
 struct AnyColumns {
     static constexpr int NU = kAnyElems / W;
     int unit, count;
+    bool full;                 // every lane of the warp has all its columns
     __device__ __forceinline__ AnyColumns(int t, int d) : unit(t / 32 * 32 * NU + t % 32) {
         const int units = d / W;
         count = unit < units ? min(NU, (units - unit + 31) / 32) : 0;
+        full = __all_sync(0xffffffffu, count == NU);
     }
     __device__ __forceinline__ int column(int k) const { return (unit + 32 * k) * W; }
     // pairs of a row in shared memory, zeros beyond the row
     template <typename T>
-    __device__ __forceinline__ void load(const T* x, F2* v) const {
+    __device__ __forceinline__ void load(const T* x, F2* v) const { full ? load_as<true>(x, v) : load_as<false>(x, v); }
+    template <bool FULL, typename T>
+    __device__ __forceinline__ void load_as(const T* x, F2* v) const {
 #pragma unroll
         for (int k = 0; k < NU; ++k) {
             RawVec<T, W> r{};
-            if (k < count) r = *reinterpret_cast<const RawVec<T, W>*>(x + unit * W + 32 * W * k);
+            if (FULL || k < count) r = *reinterpret_cast<const RawVec<T, W>*>(x + unit * W + 32 * W * k);
             float f[2];
             unpack<T, W>(r, f);
             put(v, k, f);
@@ -533,18 +537,27 @@ struct AnyColumns {
         else f[0] = k & 1 ? x.y : x.x;
     }
     template <typename T>
-    __device__ __forceinline__ void store(T* y, const F2* v) const {
+    __device__ __forceinline__ void store(T* y, const F2* v) const { full ? store_as<true>(y, v) : store_as<false>(y, v); }
+    template <bool FULL, typename T>
+    __device__ __forceinline__ void store_as(T* y, const F2* v) const {
 #pragma unroll
         for (int k = 0; k < NU; ++k) {
             float f[2];
             get(v, k, f);
-            if (k < count) *reinterpret_cast<RawVec<T, W>*>(y + unit * W + 32 * W * k) = pack<T, W>(f);
+            if (FULL || k < count) *reinterpret_cast<RawVec<T, W>*>(y + unit * W + 32 * W * k) = pack<T, W>(f);
         }
     }
-    // 1 in the columns of the row, 0 beyond
-    __device__ __forceinline__ F2 mask(int j) const {
-        if constexpr (W == 2) return f2(j < count ? 1.f : 0.f);
-        else return f2(2 * j < count ? 1.f : 0.f, 2 * j + 1 < count ? 1.f : 0.f);
+    // v - mean in the columns of the row; beyond it zeros stay zeros
+    __device__ __forceinline__ void center(F2* v, float mean) const {
+        const F2 minus = f2(-mean);
+        if (full) {
+#pragma unroll
+            for (int j = 0; j < kAnyElems / 2; ++j) v[j] = f2_add(v[j], minus);
+        } else {
+#pragma unroll
+            for (int j = 0; j < kAnyElems / 2; ++j)
+                v[j] = f2_add(v[j], W == 2 ? f2(j < count ? -mean : 0.f) : f2(2 * j < count ? -mean : 0.f, 2 * j + 1 < count ? -mean : 0.f));
+        }
     }
     template <typename T>
     __device__ __forceinline__ void params(const NormArgs& a, const void* p, float missing, F2* v) const {
@@ -596,12 +609,9 @@ norm_forward_any_kernel(NormArgs a) {
 #pragma unroll
         for (int j = 0; j < E / 2; ++j) sum = f2_add(sum, v[j]);
         const float mean = group_sum(f2_total(sum), p, share) * per_d;
-        const F2 minus = f2(-mean);
+        mine.center(v, mean);
 #pragma unroll
-        for (int j = 0; j < E / 2; ++j) {
-            v[j] = f2_fma(minus, mine.mask(j), v[j]);     // beyond the row: zeros stay zeros
-            m2 = f2_fma(v[j], v[j], m2);
-        }
+        for (int j = 0; j < E / 2; ++j) m2 = f2_fma(v[j], v[j], m2);
         const float rstd = 1.f / sqrtf(fmaf(group_sum(f2_total(m2), p, share + kShare), per_d, a.eps));
         share = (it & 1) ? share - 2 * kShare : share + 2 * kShare;
         if (p.t == 0) {
@@ -693,9 +703,10 @@ norm_backward_any_kernel(NormArgs a) {
             }
         } else {
             mine.load(x, h);
-            const F2 minus = f2(-mean), r2 = f2(rstd);
+            const F2 r2 = f2(rstd);
+            mine.center(h, mean);
 #pragma unroll
-            for (int j = 0; j < E / 2; ++j) h[j] = f2_mul(f2_fma(minus, mine.mask(j), h[j]), r2);
+            for (int j = 0; j < E / 2; ++j) h[j] = f2_mul(h[j], r2);
         }
         F2 s1 = f2(0.f), s2 = f2(0.f);
 #pragma unroll
