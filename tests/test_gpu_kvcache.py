@@ -283,3 +283,33 @@ def test_graph_replay(gpu):
             for (x, s), (_, _, _, out, _) in zip(new, sets):
                 for o in out:
                     assert np.array_equal(o.to_host()[:, :, s - 1, 0].astype(np.float64), kept(x.astype(np.float64), "int8"))
+
+
+def test_strided_indices_and_value_heads(gpu):
+    """Slots, positions, pages and lengths as strided views; values of another head size; many heads, whose
+    vectors of one token are more than a block's threads."""
+    rng = np.random.default_rng(17)
+    for dk, dv, heads in ((64, 32, 2), (128, 128, 40), (256, 64, 33)):
+        cache = gpu.quantized_cache(dk, heads, 8, 6, value_dim=dv)
+        n = 11
+        K, V = rng.standard_normal((dk, heads, n)).astype(np.float32), rng.standard_normal((dv, heads, n)).astype(np.float32)
+        slots = rng.permutation(48)[:n] + 1
+        wide = np.zeros((3, n), np.int64)
+        wide[1] = slots
+        S = gpu.ROCArray.from_host(wide).subview(1, slice(None))
+        gpu.cache_write_(cache, gpu.ROCArray.from_host(K), gpu.ROCArray.from_host(V), S)
+        pages = np.zeros((2, 5, 3), np.int32)
+        pages[1, :3, 1:] = np.array([[1, 6], [2, 5], [4, 3]])
+        lengths = np.zeros((4, 2), np.int32)
+        lengths[2] = [20, 24]
+        out = [gpu.zeros(np.float32, (d, heads, 24, 2)) for d in (dk, dv)]
+        gpu.cache_read_(*out, cache, gpu.ROCArray.from_host(pages).subview(1, slice(0, 3), slice(1, 3)), gpu.ROCArray.from_host(lengths).subview(2, slice(None)))
+        gpu.synchronize()
+        for o, x in zip(out, (K, V)):
+            full = np.zeros((x.shape[0], heads, 48))
+            full[:, :, slots - 1] = kept(x.astype(np.float64), "int8")
+            h = o.to_host()
+            for b, (table, m) in enumerate((([1, 2, 4], 20), ([6, 5, 3], 24))):
+                l = np.arange(m)
+                row = (np.array(table)[l // 8] - 1) * 8 + l % 8
+                assert np.array_equal(h[:, :, :m, b], full[:, :, row]) and not h[:, :, m:, b].any()

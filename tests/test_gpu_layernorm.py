@@ -281,3 +281,47 @@ def test_streams_threads_and_graphs(gpu):
         for a, w in zip(eager, sets[0][4]):
             assert bits_equal(a.to_host(), w)
     st.synchronize()
+
+
+def test_unaligned_parameters_and_broadcast_gradients(gpu):
+    """Parameters off 16 bytes beside aligned rows, a gradient that is one row for all (row stride 0), and
+    gradients asked for one by one."""
+    rng = np.random.default_rng(21)
+    for t in ref.TYPES.values():
+        for p in (np.dtype(np.float32), t):
+            for d, n in ((512, 7), (4096, 5), (1023, 6), (390, 9)):
+                x = rows(rng, d, n, t)
+                gamma, beta = params(rng, d, p)
+                G = gpu.ROCArray.from_host(np.concatenate([gamma[:1], gamma])).view(1, d + 1)
+                B = gpu.ROCArray.from_host(np.concatenate([beta[:1], beta])).view(1, d + 1)
+                X = gpu.ROCArray.from_host(x)
+                M, R = gpu.ROCArray(np.float32, n), gpu.ROCArray(np.float32, n)
+                Y = gpu.layernorm_(X.similar(), X, G, B, eps=EPS, mean=M, rstd=R)
+                check_forward(gpu, x, gamma, beta, Y.to_host(), M.to_host(), R.to_host(), what=(d, n))
+                one = rng.standard_normal(d).astype(t)
+                buf = gpu.ROCArray.from_host(one)
+                DY = gpu.ROCArray(t, (d, n), _buf=buf.buf, _strides=(1, 0))
+                dy = np.repeat(one[:, None], n, axis=1)
+                mean, rstd = M.to_host().astype(np.float64), R.to_host().astype(np.float64)
+                hat = (x.astype(np.float64) - mean) * rstd
+                DX, DG, DB = gpu.ROCArray(t, (d, n)), gpu.ROCArray(p, d), gpu.ROCArray(p, d)
+                gpu.layernorm_backward_(DX, DY, X, G, mean=M, rstd=R, dgamma=DG)
+                gpu.layernorm_backward_(None, DY, X, G, mean=M, rstd=R, dbeta=DB)
+                check_backward(hat, rstd, dy, gamma, DX.to_host(), DG.to_host(), DB.to_host(), 2 * U * np.abs(hat), (d, n))
+    gpu.synchronize()
+
+
+def test_rows_over_several_streams(gpu):
+    """Operators on two streams by turns, on the same arrays: each waits for what the other wrote."""
+    rng = np.random.default_rng(22)
+    d, n = 2048, 3000
+    x = rows(rng, d, n, ref.BF16)
+    X = gpu.ROCArray.from_host(x)
+    a, b = gpu.Stream(), gpu.Stream()
+    want = gpu.layernorm(gpu.layernorm(gpu.layernorm(X))).to_host()
+    Y, Z, W = (X.similar() for _ in range(3))
+    for _ in range(3):
+        gpu.layernorm_(Y, X, stream=a)
+        gpu.layernorm_(Z, Y, stream=b)
+        gpu.layernorm_(W, Z, stream=a)
+        assert bits_equal(W.to_host(), want)
