@@ -380,8 +380,8 @@ extern "C" int32_t b200_cache_write(b200_stream_t st, const b200_tensor* KQ, con
                                     const b200_tensor* positions, const b200_tensor* table, int32_t layout, double factor) {
     CacheArgs a{};
     B200_TRY(cache_pair(KQ, KS, VQ, VS, &a));
-    B200_TRY(no_overlap(KQ, "cache keys"));
-    B200_TRY(no_overlap(VQ, "cache values"));
+    for (const b200_tensor* t : {KQ, KS}) B200_TRY(no_overlap(t, "cache keys"));
+    for (const b200_tensor* t : {VQ, VS}) B200_TRY(no_overlap(t, "cache values"));
     int32_t dtype = -1;
     B200_TRY(cache_rows(K, KQ, 3, "cache write keys", &dtype));
     B200_TRY(cache_rows(V, VQ, 3, "cache write values", &dtype));
@@ -513,7 +513,7 @@ extern "C" int32_t b200_cache_read(b200_stream_t st, const b200_tensor* K, const
     attr[0].val.programmaticStreamSerializationAllowed = overlap_launches_enabled() ? 1 : 0;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    B200_CUDA(by_row_type(dtype, v, [&](auto t, auto w) { 
+    B200_CUDA(by_row_type(dtype, v, [&](auto t, auto w) {
         using T = decltype(t);
         constexpr int W = decltype(w)::value;
         return a.e4m3 ? cudaLaunchKernelEx(&cfg, cache_read_kernel<T, W, kE4M3>, a) : cudaLaunchKernelEx(&cfg, cache_read_kernel<T, W, kInt8>, a);

@@ -1,8 +1,9 @@
 /*
  * b200arrays.h — C ABI of libb200arrays.so: hand-written sm_100a CUDA kernels for the dense
  * data-parallel array path of AMDGPU.jl (fused broadcast, mapreduce with dims, accumulate,
- * sort/sortperm) together with the stream-ordered memory pool and the stream/event runtime
- * those operators sit on.
+ * sort/sortperm) and for the row operators of a transformer block that users compose from it
+ * (layer norm, 8-bit activation checkpoints, rotary positions, a quantised cache), together with
+ * the stream-ordered memory pool and the stream/event runtime those operators sit on.
  *
  * Conventions (they follow the reference's FFI layer: gen/hip/generator.jl:44-70 wraps every
  * driver call in a status check, src/hip/error.jl:143-147 treats "not ready" as a non-error):
@@ -299,7 +300,8 @@ int32_t b200_fill_random(b200_stream_t st, const b200_tensor* out, int32_t dist,
  * Y = (X - m) r gamma + beta, m = mean, r = 1/sqrt(variance + eps) of each row.  gamma and beta hold
  * one value per element of a row, both Float32 or both of X's type; either may be NULL.  mean, rstd:
  * NULL, or Float32, one per row, for the gradient.  Q, S: NULL, or receive the rows (X - m) r in
- * 8 bits (lead must be 1), which the gradient takes instead of X and mean.  Rows are dense and may be
+ * 8 bits (lead must be 1), which the gradient takes instead of X and mean; codes that did not come from
+ * here must hold magnitudes below 2^73.  Rows are dense and may be
  * any one distance apart. */
 int32_t b200_layernorm(b200_stream_t st, const b200_tensor* Y, const b200_tensor* X, int32_t lead,
                        const b200_tensor* gamma, const b200_tensor* beta, double eps,

@@ -175,6 +175,18 @@ def test_cache_arguments(pkg):
         pkg.cache_write_(pkg.QuantizedCache(pkg.Quantized8.wrap(kq, ks), pkg.Quantized8.wrap(vq, vs)), k, v, sl, positions=sl)
 
 
+def test_cache_scales_that_overlap(pkg):
+    """Scale bytes of two heads, places or pages in one place are refused like codes are."""
+    f = lambda *a, **k: fake(pkg, *a, **k)
+    k, sl = f(np.float32, (64, 2, 7)), f(np.int64, (7,))
+    q, s = f(np.int8, (64, 2, 16, 5)), f(np.uint8, (2, 2, 16, 5))
+    assert_valid(pkg, "b200_cache_write", q, s, q, s, k, k, sl, None, None, 0, 1.0)
+    for strides in ((1, 0, 4, 64), (1, 1, 4, 64), (1, 2, 0, 64), (1, 2, 4, 1)):
+        bad = f(np.uint8, (2, 2, 16, 5), strides=strides)
+        assert_refused(pkg, pkg._lib.INVALID_ARG, "overlap", "b200_cache_write", q, bad, q, s, k, k, sl, None, None, 0, 1.0)
+        assert_refused(pkg, pkg._lib.INVALID_ARG, "overlap", "b200_cache_write", q, s, q, bad, k, k, sl, None, None, 0, 1.0)
+
+
 def test_python_checks(pkg):
     f = lambda *a, **k: fake(pkg, *a, **k)
     x = f(np.float32, (8, 3))
