@@ -18,7 +18,7 @@ struct NormArgs {
     float *partial;                     // gradient: [block][2][d] sums of dy*h and dy
     int64_t ldx, ldy, lddy, rows, d, blocks;
     // ring kernels: rows from one of a group's to its next, and that many rows of each array in elements
-    int64_t step, x_step, y_step, dy_step, q_step;
+    int64_t step, x_step, y_step, dy_step, q_step, s_step;
     float eps;
     int32_t gamma_f32, e4m3, group;     // group: threads per row
     int32_t pitch, pitch_x, units2;     // rows of any alignment: bytes of a stage of the rings; two elements at a time
@@ -50,9 +50,14 @@ __device__ __forceinline__ float lane_sum(float v, int width) {
 // With the loads out of the way these kernels are bound by instruction issue, not by HBM: arithmetic goes
 // in pairs (F2), a thread has as many columns as its registers hold, and nothing is predicated but the
 // copies and stores (vectors beyond a row read as zeros).  One B200, 16384 x 4096 BFloat16: forward 48 us
-// (5.5 TB/s), with the 8-bit rows written as well 61 us, gradient 69 us (5.8 TB/s), from the 8-bit rows
-// 72 us; waiting for each row in turn the gradient takes 120 us.  A register spilled inside the loop costs
+// (5.5 TB/s), with the 8-bit rows written as well 63 us, gradient 69 us (5.8 TB/s), from the 8-bit rows
+// 66 us; waiting for each row in turn the gradient takes 120 us.  A register spilled inside the loop costs
 // more than a second pass over it (20 bytes: 69 -> 84 us).
+//
+// FULL: rows that fill every thread of whole warps (d = group * E).  A warp's vectors lie side by side there,
+// so that a thread's steps through a row are known at compile time, and nothing is predicated: 8192 x 5120
+// BFloat16 forward with the 8-bit rows 41 us (44 without), gradient from them 50 us (56), 8192 x 6144 Float16
+// 46 (55) and 55 (61) us, 8192 x 8192 gradient 79 (84) us; 16384 x 4096 forward with the 8-bit rows 63 (61) us.
 
 enum { kAsIs = 0 };                     // form of the rows kept for the gradient: as they are, kInt8, kE4M3
 
@@ -127,11 +132,11 @@ __device__ __forceinline__ void ring_copy(void* dst, const void* src) {
     else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(d), "l"(src), "n"(BYTES) : "memory");
 }
 template <typename T, int V, int NV>
-__device__ __forceinline__ void load_params2(const NormArgs& a, const void* p, int t, int nvec, float missing, F2* out) {
+__device__ __forceinline__ void load_params2(const NormArgs& a, const void* p, int t, int step, int nvec, float missing, F2* out) {
     const bool aligned = (reinterpret_cast<uintptr_t>(p) & 15) == 0;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-        const int vi = t + k * a.group;
+        const int vi = t + k * step;
 #pragma unroll
         for (int i = 0; i < V / 2; ++i) out[k * V / 2 + i] = f2(missing);
         if (!p || vi >= nvec) continue;
@@ -158,7 +163,7 @@ __device__ __forceinline__ void load_params2(const NormArgs& a, const void* p, i
 }
 
 // Two passes over the row in registers: the mean first, then the squares about it.
-template <typename T, int E, int STAGES, int THREADS, int KEEP>
+template <typename T, int E, int STAGES, int THREADS, int KEEP, bool FULL>
 __global__ void __launch_bounds__(THREADS)
 norm_forward_ring_kernel(NormArgs a) {
     constexpr int V = 16 / (int)sizeof(T), NV = E / V, SLOT = NV * THREADS;
@@ -168,19 +173,21 @@ norm_forward_ring_kernel(NormArgs a) {
     __syncthreads();
     grid_dependency_wait();
     const RingPlace p(a.group, a.rows, a.step);
-    const int G = a.group, t = p.t, nvec = (int)(a.d / V);
+    const int S = FULL ? 32 : a.group, t = FULL ? p.warp * (32 * NV) + p.lane : p.t, nvec = (int)(a.d / V);
     bool in[NV];
 #pragma unroll
-    for (int k = 0; k < NV; ++k) in[k] = t + k * G < nvec;
+    for (int k = 0; k < NV; ++k) in[k] = FULL || t + k * S < nvec;
     const T* src = reinterpret_cast<const T*>(a.x) + p.row * a.ldx + (int64_t)t * V;      // next row to fetch
     T* dst = reinterpret_cast<T*>(a.y) + p.row * a.ldy + (int64_t)t * V;
+    uint8_t* dst_q = a.q + p.row * a.d + t * V;
+    uint8_t* dst_s = a.s + p.row * a.blocks + t / (kBlock / V);
     uint4* own = ring + threadIdx.x;
     int to_fetch = p.mine;
     auto fetch = [&](int slot) {
         if (to_fetch > 0) {
 #pragma unroll
             for (int k = 0; k < NV; ++k)
-                if (in[k]) ring_copy<16>(own + slot + k * THREADS, src + k * G * V);
+                if (in[k]) ring_copy<16>(own + slot + k * THREADS, src + k * S * V);
         }
         --to_fetch;
         src += a.x_step;
@@ -195,14 +202,14 @@ norm_forward_ring_kernel(NormArgs a) {
 #pragma unroll
     for (int s = 0; s < STAGES - 1; ++s) fetch(s * SLOT);
     F2 gm[E / 2], bt[E / 2];
-    load_params2<T, V, NV>(a, a.gamma, t, nvec, 1.f, gm);
-    load_params2<T, V, NV>(a, a.beta, t, nvec, 0.f, bt);
+    load_params2<T, V, NV>(a, a.gamma, t, S, nvec, 1.f, gm);
+    load_params2<T, V, NV>(a, a.beta, t, S, nvec, 0.f, bt);
     const float per_d = 1.f / (float)a.d;
     int slot = 0, free_slot = (STAGES - 1) * SLOT;
     float* share = &shares[p.warps > 1 ? p.group : 0][0][0];
     int64_t row = p.row;
     for (int it = 0; it < p.walk; ++it, row += a.step) {
-        const bool live = it < p.mine;
+        const bool live = FULL || it < p.mine;
         cp_async_wait<STAGES - 2>();
         F2 v[E / 2];
         F2 sum2 = f2(0.f);
@@ -230,7 +237,7 @@ norm_forward_ring_kernel(NormArgs a) {
         const float var = group_sum(f2_total(m2), p, share + kShare) * per_d;
         share = (it & 1) ? share - 2 * kShare : share + 2 * kShare;
         const float rstd = 1.f / sqrtf(var + a.eps);
-        if (live && t == 0) {
+        if (live && p.t == 0) {
             if (a.mean) a.mean[row] = mean;
             if (a.rstd) a.rstd[row] = rstd;
         }
@@ -244,23 +251,23 @@ norm_forward_ring_kernel(NormArgs a) {
                 h[i] = f2_mul(h[i], r2);
                 o[i] = f2_fma(h[i], gm[k * V / 2 + i], bt[k * V / 2 + i]);
             }
-            if (live && in[k]) st_raw<T, V>(dst + k * G * V, pack2<T, V>(o));
+            if (live && in[k]) st_raw<T, V>(dst + k * S * V, pack2<T, V>(o));
             if constexpr (KEEP != kAsIs) {
                 const uint32_t e = scale_byte(block_amax2<V>(h, live && in[k]), KEEP == kE4M3);
                 if (live && in[k]) {
-                    const int vi = t + k * G;
-                    st_raw<uint8_t, V>(a.q + row * a.d + (int64_t)vi * V, encode2<V>(h, e, KEEP == kE4M3));
-                    if (vi % (kBlock / V) == 0) a.s[row * a.blocks + vi / (kBlock / V)] = (uint8_t)e;
+                    st_raw<uint8_t, V>(dst_q + k * S * V, encode2<V>(h, e, KEEP == kE4M3));
+                    if (t % (kBlock / V) == 0) dst_s[k * (S / (kBlock / V))] = (uint8_t)e;
                 }
             }
         }
         dst += a.y_step;
+        if constexpr (KEEP != kAsIs) { dst_q += a.q_step; dst_s += a.s_step; }
     }
 }
 
 // dx needs the row again after its sums: g gamma and h stay in registers (HOLD), or the row is read out
 // of the ring a second time and the registers are for the column sums of more columns.
-template <typename T, int E, int STAGES, int THREADS, int KEPT, bool HOLD>
+template <typename T, int E, int STAGES, int THREADS, int KEPT, bool HOLD, bool FULL>
 __global__ void __launch_bounds__(THREADS)
 norm_backward_ring_kernel(NormArgs a) {
     constexpr int V = 16 / (int)sizeof(T), NV = E / V, SLOT = NV * THREADS;
@@ -271,10 +278,10 @@ norm_backward_ring_kernel(NormArgs a) {
     __syncthreads();
     grid_dependency_wait();
     const RingPlace p(a.group, a.rows, a.step);
-    const int G = a.group, t = p.t, nvec = (int)(a.d / V), per_block = blockDim.x / G;
+    const int S = FULL ? 32 : a.group, t = FULL ? p.warp * (32 * NV) + p.lane : p.t, nvec = (int)(a.d / V), per_block = blockDim.x / a.group;
     bool in[NV];
 #pragma unroll
-    for (int k = 0; k < NV; ++k) in[k] = t + k * G < nvec;
+    for (int k = 0; k < NV; ++k) in[k] = FULL || t + k * S < nvec;
     const T* src = reinterpret_cast<const T*>(a.dy) + p.row * a.lddy + (int64_t)t * V;    // next row to fetch
     const T* src_x = reinterpret_cast<const T*>(a.x) + p.row * a.ldx + (int64_t)t * V;
     const uint8_t* src_q = a.q + p.row * a.d + (int64_t)t * V;
@@ -286,9 +293,9 @@ norm_backward_ring_kernel(NormArgs a) {
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
                 if (in[k]) {
-                    ring_copy<16>(own + slot + k * THREADS, src + k * G * V);
-                    if constexpr (KEPT != kAsIs) ring_copy<V>(own_q + slot + k * THREADS, src_q + k * G * V);
-                    else ring_copy<16>(own_x + slot + k * THREADS, src_x + k * G * V);
+                    ring_copy<16>(own + slot + k * THREADS, src + k * S * V);
+                    if constexpr (KEPT != kAsIs) ring_copy<V>(own_q + slot + k * THREADS, src_q + k * S * V);
+                    else ring_copy<16>(own_x + slot + k * THREADS, src_x + k * S * V);
                 }
             }
         }
@@ -308,19 +315,21 @@ norm_backward_ring_kernel(NormArgs a) {
     }
 #pragma unroll
     for (int s = 0; s < STAGES - 1; ++s) fetch(s * SLOT, s < p.mine);
-    // gamma lies in shared memory, [vector][quarter][thread of a group]: the registers are taken
-    float4* gammas = reinterpret_cast<float4*>(reinterpret_cast<char*>(ring) + (size_t)STAGES * SLOT * (16 + (KEPT ? V : 16))) + t;
+    // gamma lies in shared memory, [vector][quarter][thread], where threads' vectors lie side by side: the
+    // registers are taken
+    float4* gammas = reinterpret_cast<float4*>(reinterpret_cast<char*>(ring) + (size_t)STAGES * SLOT * (16 + (KEPT ? V : 16))) +
+                     (FULL ? p.warp * (32 * E / 4) + p.lane : t);
     if (p.group == 0) {
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
 #pragma unroll
             for (int j = 0; j < V / 4; ++j) {
-                const int64_t c = (int64_t)(t + k * G) * V + 4 * j;
+                const int64_t c = (int64_t)(t + k * S) * V + 4 * j;
                 float4 g = make_float4(1.f, 1.f, 1.f, 1.f);
                 if (a.gamma && in[k])
                     g = make_float4(load_param(a.gamma, a.gamma_f32, dtype_of<T>(), c), load_param(a.gamma, a.gamma_f32, dtype_of<T>(), c + 1),
                                     load_param(a.gamma, a.gamma_f32, dtype_of<T>(), c + 2), load_param(a.gamma, a.gamma_f32, dtype_of<T>(), c + 3));
-                gammas[(k * (V / 4) + j) * G] = g;
+                gammas[(k * (V / 4) + j) * S] = g;
             }
         }
     }
@@ -340,7 +349,7 @@ norm_backward_ring_kernel(NormArgs a) {
             else {
                 const uint8_t* at = a.s + r * a.blocks + t / (kBlock / V);
 #pragma unroll
-                for (int k = 0; k < NV; ++k) if (in[k]) scale[k] = at[k * G / (kBlock / V)];
+                for (int k = 0; k < NV; ++k) if (in[k]) scale[k] = at[k * S / (kBlock / V)];
             }
         }
     };
@@ -348,7 +357,7 @@ norm_backward_ring_kernel(NormArgs a) {
     int slot = 0, free_slot = (STAGES - 1) * SLOT;
     float2* share = &shares[p.warps > 1 ? p.group : 0][0][0];
     for (int it = 0; it < p.walk; ++it, row += (int)a.step) {
-        const bool live = it < p.mine;
+        const bool live = it < p.mine;                    // FULL: always; without the branch the loads below move about and spill
         const float rstd = rstd_next;
         const F2 r2 = f2(rstd), minus = f2(-mean_next);
         cp_async_wait<STAGES - 2>();
@@ -373,7 +382,7 @@ norm_backward_ring_kernel(NormArgs a) {
                 load_h(k, h);
 #pragma unroll
                 for (int q = 0; q < V / 4; ++q) {
-                    const ulonglong2 gm = *reinterpret_cast<const ulonglong2*>(gammas + (k * (V / 4) + q) * G);
+                    const ulonglong2 gm = *reinterpret_cast<const ulonglong2*>(gammas + (k * (V / 4) + q) * S);
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         const int i = 2 * q + e, j = k * V / 2 + i;
@@ -404,7 +413,7 @@ norm_backward_ring_kernel(NormArgs a) {
                     load_dy(k, g);
 #pragma unroll
                     for (int q = 0; q < V / 4; ++q) {
-                        const ulonglong2 gm = *reinterpret_cast<const ulonglong2*>(gammas + (k * (V / 4) + q) * G);
+                        const ulonglong2 gm = *reinterpret_cast<const ulonglong2*>(gammas + (k * (V / 4) + q) * S);
                         g[2 * q] = f2_mul(g[2 * q], gm.x);
                         g[2 * q + 1] = f2_mul(g[2 * q + 1], gm.y);
                     }
@@ -412,7 +421,7 @@ norm_backward_ring_kernel(NormArgs a) {
                 F2 o[V / 2];
 #pragma unroll
                 for (int i = 0; i < V / 2; ++i) o[i] = f2_fma(h[i], c2, f2_fma(g[i], r2, c1));
-                if (live && in[k]) st_raw<T, V>(dst + k * G * V, pack2<T, V>(o));
+                if (live && in[k]) st_raw<T, V>(dst + k * S * V, pack2<T, V>(o));
             }
         }
         if constexpr (!HOLD) {
@@ -431,7 +440,7 @@ norm_backward_ring_kernel(NormArgs a) {
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-        float* c = column + (int64_t)p.group * d2 + (t + k * G) * V;
+        float* c = column + (int64_t)p.group * d2 + (t + k * S) * V;
         if (in[k]) {
 #pragma unroll
             for (int i = 0; i < V / 2; ++i) {             // in pairs: quads would tie the loop's registers
@@ -935,6 +944,8 @@ static int norm_vector(const NormArgs& a, int32_t dtype, bool aligned) {
     const int v = dtype == B200_F32 ? 4 : 8;
     return aligned && a.d % v == 0 && a.rows <= 0x3fffffff ? v : 1;    // the ring kernels count rows in 32 bits
 }
+// Whole warps that have all their columns: nothing is predicated.
+static bool full_rows(const NormArgs& a, int e) { return a.group % 32 == 0 && a.d == (int64_t)a.group * e; }
 // Dynamic shared memory that with the static one may pass 48 KB has to be allowed once per kernel and device.
 static cudaError_t allow_shared(const void* kernel, size_t bytes, int dev) {
     if (bytes <= 32 * 1024) return cudaSuccess;
@@ -964,7 +975,7 @@ struct NormLaunch {
     template <typename K> cudaError_t go(K kernel) {
         a.step = (int64_t)grid * (threads / a.group);
         a.x_step = a.step * a.ldx; a.y_step = a.step * a.ldy; a.dy_step = a.step * a.lddy;
-        a.q_step = a.step * a.d;
+        a.q_step = a.step * a.d; a.s_step = a.step * a.blocks;
         return launch_overlapped(kernel, grid, threads, smem, st->s, a);
     }
 };
@@ -976,8 +987,12 @@ static cudaError_t forward_ring(b200_stream_t st, const NormArgs& a) {
     while (per > 1 && a.rows < (int64_t)per * sm_count(st->dev) && (per / 2) * a.group >= 32) per /= 2;      // few rows: an SM each
     const size_t bytes = (size_t)STAGES * (E * sizeof(T)) * THREADS;
     auto run = [&](auto kernel) { const cudaError_t e = l.plan(kernel, per, bytes); return e == cudaSuccess ? l.go(kernel) : e; };
-    if (!a.q) return run(norm_forward_ring_kernel<T, E, STAGES, THREADS, kAsIs>);
-    return a.e4m3 ? run(norm_forward_ring_kernel<T, E, STAGES, THREADS, kE4M3>) : run(norm_forward_ring_kernel<T, E, STAGES, THREADS, kInt8>);
+    auto form = [&](auto full) {
+        constexpr bool FULL = decltype(full)::value;
+        if (!a.q) return run(norm_forward_ring_kernel<T, E, STAGES, THREADS, kAsIs, FULL>);
+        return a.e4m3 ? run(norm_forward_ring_kernel<T, E, STAGES, THREADS, kE4M3, FULL>) : run(norm_forward_ring_kernel<T, E, STAGES, THREADS, kInt8, FULL>);
+    };
+    return full_rows(a, E) ? form(std::true_type{}) : form(std::false_type{});
 }
 template <typename T>
 static cudaError_t run_forward(b200_stream_t st, NormArgs a, int v) {
@@ -1014,11 +1029,13 @@ static int32_t backward_ring(NormLaunch& l, F space) {
     size_t bytes = (size_t)STAGES * (E / V) * (16 + (KEPT ? V : 16)) * THREADS + (size_t)E * l.a.group * sizeof(float);
     const size_t columns = (size_t)per * 2 * l.a.d * sizeof(float);
     if (bytes < columns) bytes = columns;
-    auto kernel = norm_backward_ring_kernel<T, E, STAGES, THREADS, KEPT, HOLD>;
-    B200_CUDA(l.plan(kernel, per, bytes));
-    B200_TRY(space((int64_t)l.grid));
-    B200_CUDA(l.go(kernel));
-    return B200_OK;
+    auto run = [&](auto kernel) -> int32_t {
+        B200_CUDA(l.plan(kernel, per, bytes));
+        B200_TRY(space((int64_t)l.grid));
+        B200_CUDA(l.go(kernel));
+        return B200_OK;
+    };
+    return full_rows(l.a, E) ? run(norm_backward_ring_kernel<T, E, STAGES, THREADS, KEPT, HOLD, true>) : run(norm_backward_ring_kernel<T, E, STAGES, THREADS, KEPT, HOLD, false>);
 }
 
 // Workspace of one call.  Outside a capture it is the stream's scratch; inside one the graph gets an
@@ -1053,8 +1070,9 @@ static int32_t run_backward(b200_stream_t st, NormArgs a, int v, void* dgamma, v
     const int g16 = ring_group(a.d, 16, v), g32 = ring_group(a.d, 32, v);
     // 32 columns per thread where that holds more rows side by side on an SM than 16 do: fewer
     // instructions per element (16384 x 4096 BFloat16: 69 us, with 16 columns 80; 8192 x 8192: 93 and 84,
-    // one row per SM either way).  Up to 2048 columns the two differ by less than 5 % either way.
-    const bool wide = k16 && v > 1 && g32 <= 384 && (g16 > 512 || (a.d > 2048 && 384 / g32 > 512 / g16));
+    // one row per SM either way).  Up to 2048 columns only where they fill the threads (16384 x 2048 out
+    // of 8 bits 38 us, with 16 columns 42; 16384 x 1536, which they do not fill, 39 and 33).
+    const bool wide = k16 && v > 1 && g32 <= 384 && (g16 > 512 || ((a.d > 2048 || a.d % 1024 == 0) && 384 / g32 > 512 / g16));
     if (wide) {
         l.a.group = g32;
         if constexpr (k16) {

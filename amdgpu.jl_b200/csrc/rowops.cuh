@@ -333,15 +333,15 @@ __device__ __forceinline__ float block_amax2(const F2* v, bool in) {
 }
 template <int V>
 __device__ __forceinline__ RawVec<uint8_t, V> encode2(const F2* v, uint32_t e, bool e4m3) {
-    RawVec<uint8_t, V> r{};
-    if (e == 255u) return r;
+    RawVec<uint8_t, V> r;
     const F2 inv = f2(inverse_scale(e));
+    const uint32_t mask = e == 255u ? 0u : ~0u;           // no branch around the rest
     uint32_t* w = reinterpret_cast<uint32_t*>(&r);
     if (e4m3) {
 #pragma unroll
         for (int i = 0; i < V / 4; ++i) {
             const float2 a = f2_parts(f2_mul(v[2 * i], inv)), b = f2_parts(f2_mul(v[2 * i + 1], inv));
-            w[i] = e4m3_pair(a.x, a.y) | e4m3_pair(b.x, b.y) << 16;
+            w[i] = (e4m3_pair(a.x, a.y) | e4m3_pair(b.x, b.y) << 16) & mask;
         }
     } else {
         const F2 magic = f2(12582912.f);
@@ -350,7 +350,7 @@ __device__ __forceinline__ RawVec<uint8_t, V> encode2(const F2* v, uint32_t e, b
             const float2 a = f2_parts(f2_fma(v[2 * i], inv, magic)), b = f2_parts(f2_fma(v[2 * i + 1], inv, magic));
             const uint32_t lo = __byte_perm(__float_as_uint(a.x), __float_as_uint(a.y), 0x0040);
             const uint32_t hi = __byte_perm(__float_as_uint(b.x), __float_as_uint(b.y), 0x0040);
-            w[i] = __byte_perm(lo, hi, 0x5410);
+            w[i] = __byte_perm(lo, hi, 0x5410) & mask;
         }
     }
     return r;
