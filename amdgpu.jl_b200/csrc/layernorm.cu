@@ -483,12 +483,16 @@ struct PieceRing {
     __device__ __forceinline__ PieceRing(const void* p, int64_t row_elems, int64_t ld_elems, int64_t rows, char* smem, int pitch_)
         : lo(reinterpret_cast<const char*>(p)), hi(lo + ((rows - 1) * ld_elems + row_elems) * (int64_t)sizeof(T)), buf(smem), pitch(pitch_),
           bytes((int)(row_elems * sizeof(T))), ld(ld_elems * (int64_t)sizeof(T)) {}
-    __device__ __forceinline__ int offset(int64_t row) const { return (int)(reinterpret_cast<uintptr_t>(lo + row * ld) & 15); }
+    __device__ __forceinline__ int offset(int64_t row) const { return ((uint32_t)reinterpret_cast<uintptr_t>(lo) + (uint32_t)row * (uint32_t)ld) & 15; }
     __device__ __forceinline__ void fetch(int64_t row, int stage, int t, int G) const {
         const char* first = lo + row * ld;
         const char* from = first - offset(row);
         char* to = buf + stage * pitch;
         const int n = (offset(row) + bytes + 15) / 16;
+        if (from >= lo && from + 16 * n <= hi) {              // all but the first and the last rows of an array
+            for (int c = t; c < n; c += G) ring_copy<16>(to + 16 * c, from + 16 * c);
+            return;
+        }
         for (int c = t; c < n; c += G) {
             const char* src = from + 16 * c;
             if (src >= lo && src + 16 <= hi) {
@@ -522,6 +526,106 @@ struct AnyColumns {
         full = __all_sync(0xffffffffu, count == NU);
     }
     __device__ __forceinline__ int column(int k) const { return (unit + 32 * k) * W; }
+    // A warp's columns are kWarpBlocks blocks of 32.  Each block's scale is one lane's work: lane k for block k,
+    // or, two columns to a unit, lanes 2 k and 2 k + 1 of either half for the half's block of unit k.
+    static constexpr int kWarpBlocks = kAnyElems;
+    static __device__ __forceinline__ int block_of_lane() {
+        const int lane = threadIdx.x % 32;
+        return W == 1 ? lane % kWarpBlocks : 2 * (lane / 2 % NU) + lane / 16;
+    }
+    static __device__ __forceinline__ int lane_of_unit(int k) { return W == 1 ? k : (int)(threadIdx.x & 16) | 2 * k; }
+    // Largest magnitude, as bits, of this lane's block.
+    __device__ __forceinline__ uint32_t block_most(const F2* v) const {
+        const int lane = threadIdx.x % 32;
+        uint32_t m[NU];
+#pragma unroll
+        for (int k = 0; k < NU; ++k) {
+            float f[2];
+            get(v, k, f);
+            m[k] = __float_as_uint(f[0]) & 0x7fffffffu;
+            if constexpr (W == 2) m[k] = max(m[k], __float_as_uint(f[1]) & 0x7fffffffu);
+        }
+        if constexpr (W == 1) {
+            uint32_t most = 0;
+#pragma unroll
+            for (int k = 0; k < NU; ++k) {
+                const uint32_t r = __reduce_max_sync(0xffffffffu, m[k]);
+                if (lane % kWarpBlocks == k) most = r;
+            }
+            return most;
+        } else {
+            // every exchange halves the units a lane carries
+#pragma unroll
+            for (int o = 8, n = NU / 2; o >= 2; o /= 2, n /= 2) {
+#pragma unroll
+                for (int k = 0; k < n; ++k) {
+                    const bool upper = lane & o;
+                    const uint32_t keep = upper ? m[k + n] : m[k], give = upper ? m[k] : m[k + n];
+                    m[k] = max(keep, __shfl_xor_sync(0xffffffffu, give, o));
+                }
+            }
+            return max(m[0], __shfl_xor_sync(0xffffffffu, m[0], 1));
+        }
+    }
+    // The row's codes and scale bytes; PLAIN: all columns are there and all blocks are finite.
+    template <bool PLAIN, bool E4M3>
+    __device__ __forceinline__ void store_codes(uint8_t* q, const F2* v, float inv) const {
+#pragma unroll
+        for (int k = 0; k < NU; ++k) {
+            const float s = __shfl_sync(0xffffffffu, inv, lane_of_unit(k));
+            float f[2] = {0.f, 0.f};
+            get(v, k, f);
+            uint32_t c;
+            if constexpr (E4M3) c = e4m3_pair(f[0] * s, f[1] * s);
+            else if constexpr (W == 1) c = int8_code(f[0], s);
+            else c = __byte_perm(int8_code(f[0], s), int8_code(f[1], s), 0x0040);
+            if (!PLAIN && s == 0.f) c = 0;
+            if (PLAIN || k < count) {
+                if constexpr (W == 1) q[unit + 32 * k] = (uint8_t)c;
+                else *reinterpret_cast<uint16_t*>(q + 2 * unit + 64 * k) = (uint16_t)c;
+            }
+        }
+    }
+    __device__ __forceinline__ void keep(uint8_t* q, uint8_t* sc, int warp, int blocks, bool e4m3, const F2* v) const {
+        const uint32_t e = scale_byte(__uint_as_float(block_most(v)), e4m3);
+        const int block = warp * kWarpBlocks + block_of_lane();
+        if ((W == 1 ? threadIdx.x % 32 < 16 : threadIdx.x % 2 == 0) && block < blocks) sc[block] = (uint8_t)e;
+        const float inv = e == 255u ? 0.f : inverse_scale(e);
+        if (__all_sync(0xffffffffu, full && e != 255u)) {
+            if (e4m3) store_codes<true, true>(q, v, inv);
+            else store_codes<true, false>(q, v, inv);
+        } else {
+            if (e4m3) store_codes<false, true>(q, v, inv);
+            else store_codes<false, false>(q, v, inv);
+        }
+    }
+    // The row out of its codes in shared memory, zeros beyond it; scale: of this lane's block.
+    template <bool E4M3>
+    __device__ __forceinline__ void restore(const uint8_t* x, float scale, F2* v) const {
+#pragma unroll
+        for (int k = 0; k < NU; k += 2 / W) {
+            uint32_t c[2] = {0, 0};
+            float s[2];
+            s[0] = s[1] = __shfl_sync(0xffffffffu, scale, lane_of_unit(k));
+            if constexpr (W == 1) {
+                s[1] = __shfl_sync(0xffffffffu, scale, lane_of_unit(k + 1));
+                if (full || k < count) c[0] = x[unit + 32 * k];
+                if (full || k + 1 < count) c[1] = x[unit + 32 * k + 32];
+            } else {
+                uint32_t w = 0;
+                if (full || k < count) w = *reinterpret_cast<const uint16_t*>(x + 2 * unit + 64 * k);
+                c[0] = w & 0xff;
+                c[1] = w >> 8;
+            }
+            if constexpr (E4M3) {
+                const float2 f = e4m3_values((uint16_t)(c[0] | c[1] << 8));
+                v[k * W / 2] = f2_mul(f2(f.x, f.y), f2(s[0], s[1]));
+            } else {                                          // as in decode: the low mantissa bits of 2^23
+                const F2 u = f2(__uint_as_float(c[0] ^ 0x4b000080u), __uint_as_float(c[1] ^ 0x4b000080u));
+                v[k * W / 2] = f2_mul(f2_add(u, f2(-8388736.f)), f2(s[0], s[1]));
+            }
+        }
+    }
     // pairs of a row in shared memory, zeros beyond the row
     template <typename T>
     __device__ __forceinline__ void load(const T* x, F2* v) const { full ? load_as<true>(x, v) : load_as<false>(x, v); }
@@ -636,29 +740,7 @@ norm_forward_any_kernel(NormArgs a) {
         }
         mine.store(reinterpret_cast<T*>(a.y) + row * a.ldy, o);
         if constexpr (KEEP) {
-            // 32 / W neighbouring lanes hold a block of 32; magnitudes compare like their bits, NaN above all
-            uint8_t* q = a.q + row * a.d + mine.unit * W;
-            uint8_t* sc = a.s + row * a.blocks + mine.unit * W / kBlock;
-#pragma unroll
-            for (int k = 0; k < mine.NU; ++k) {
-                if (mine.column(k) - p.t % 32 * W >= (int)a.d) break;      // the same for the whole warp
-                float f[2] = {0.f, 0.f};
-                mine.get(v, k, f);
-                uint32_t m = __float_as_uint(f[0]) & 0x7fffffffu;
-                if constexpr (W == 2) {
-                    m = max(m, __float_as_uint(f[1]) & 0x7fffffffu);
-#pragma unroll
-                    for (int o = 8; o > 0; o /= 2) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-                } else {
-                    m = __reduce_max_sync(0xffffffffu, m);
-                }
-                const uint32_t e = scale_byte(__uint_as_float(m), a.e4m3);
-                if (k < mine.count) {
-                    if constexpr (W == 2) *reinterpret_cast<uint16_t*>(q + 32 * W * k) = (uint16_t)(encode<1>(f, e, a.e4m3) | encode<1>(f + 1, e, a.e4m3) << 8);
-                    else q[32 * k] = encode<1>(f, e, a.e4m3);
-                    if (p.t % (kBlock / W) == 0) sc[W * k] = (uint8_t)e;
-                }
-            }
+            mine.keep(a.q + row * a.d, a.s + row * a.blocks, p.warp, (int)a.blocks, a.e4m3, v);
         }
     }
 }
@@ -691,25 +773,29 @@ norm_backward_any_kernel(NormArgs a) {
     const float per_d = 1.f / (float)a.d;
     float2* share = &shares[p.warps > 1 ? p.group : 0][0][0];
     int stage = 0, row = (int)p.row;
+    // what a row needs beside the rings is loaded one row ahead
+    const int block = p.warp * AnyColumns<W>::kWarpBlocks + AnyColumns<W>::block_of_lane();
+    float rstd_next = 0.f, mean_next = 0.f;
+    uint32_t scale_next = 0;
+    auto ahead = [&](int r, bool live) {
+        if (!live) return;
+        rstd_next = a.rstd[r];
+        if constexpr (!KEPT) mean_next = a.mean[r];
+        else if (block < (int)a.blocks) scale_next = a.s[r * a.blocks + block];
+    };
+    ahead(row, p.mine > 0);
     for (int it = 0; it < p.mine; ++it, row += (int)a.step) {
-        const float rstd = a.rstd[row], mean = KEPT ? 0.f : a.mean[row];
+        const float rstd = rstd_next, mean = mean_next;
+        const uint32_t scale = scale_next;
+        ahead(row + (int)a.step, it + 1 < p.mine);
         cp_async_wait<kAnyStages - 2>();
         group_sync(p);
         F2 g[E / 2], h[E / 2];
         mine.load(ring.row(row, stage), g);
         const S* x = ring_x.row(row, stage);
         if constexpr (KEPT) {
-            const uint8_t* sc = a.s + row * a.blocks + mine.unit * W / kBlock;
-#pragma unroll
-            for (int k = 0; k < mine.NU; ++k) {
-                float f[2] = {0.f, 0.f};
-                if (k < mine.count) {
-                    const uint32_t e = sc[W * k];
-#pragma unroll
-                    for (int i = 0; i < W; ++i) decode<1>(x[mine.unit * W + 32 * W * k + i], e, a.e4m3, f + i);
-                }
-                mine.put(h, k, f);
-            }
+            if (a.e4m3) mine.template restore<true>(x, scale_value(scale), h);
+            else mine.template restore<false>(x, scale_value(scale), h);
         } else {
             mine.load(x, h);
             const F2 r2 = f2(rstd);
