@@ -515,9 +515,9 @@ __device__ __forceinline__ void group_sync(const RingPlace& p) {
 // A thread's columns: units of W neighbours, its warp's first unit + lane + 32 k for k < count (steps known
 // at compile time: no registers for addresses); W is 2 where every row of 16-bit elements starts on 4 bytes.
 // Two elements to a pair: those of a unit, or those of units 2j, 2j+1.
-template <int W>
+template <int W, int E>
 struct AnyColumns {
-    static constexpr int NU = kAnyElems / W;
+    static constexpr int NU = E / W;
     int unit, count;
     bool full;                 // every lane of the warp has all its columns
     __device__ __forceinline__ AnyColumns(int t, int d) : unit(t / 32 * 32 * NU + t % 32) {
@@ -527,13 +527,13 @@ struct AnyColumns {
     }
     __device__ __forceinline__ int column(int k) const { return (unit + 32 * k) * W; }
     // A warp's columns are kWarpBlocks blocks of 32.  Each block's scale is one lane's work: lane k for block k,
-    // or, two columns to a unit, lanes 2 k and 2 k + 1 of either half for the half's block of unit k.
-    static constexpr int kWarpBlocks = kAnyElems;
+    // or, two columns to a unit, the 16 / NU lanes from k 16 / NU on of either half for the half's block of unit k.
+    static constexpr int kWarpBlocks = E, kLanes = W == 1 ? 1 : 16 / NU;
     static __device__ __forceinline__ int block_of_lane() {
         const int lane = threadIdx.x % 32;
-        return W == 1 ? lane % kWarpBlocks : 2 * (lane / 2 % NU) + lane / 16;
+        return W == 1 ? lane % kWarpBlocks : 2 * (lane % 16 / kLanes) + lane / 16;
     }
-    static __device__ __forceinline__ int lane_of_unit(int k) { return W == 1 ? k : (int)(threadIdx.x & 16) | 2 * k; }
+    static __device__ __forceinline__ int lane_of_unit(int k) { return W == 1 ? k : (int)(threadIdx.x & 16) | kLanes * k; }
     // Largest magnitude, as bits, of this lane's block.
     __device__ __forceinline__ uint32_t block_most(const F2* v) const {
         const int lane = threadIdx.x % 32;
@@ -554,9 +554,10 @@ struct AnyColumns {
             }
             return most;
         } else {
-            // every exchange halves the units a lane carries
+            // every exchange halves the units a lane carries, until one is left
 #pragma unroll
-            for (int o = 8, n = NU / 2; o >= 2; o /= 2, n /= 2) {
+            for (int o = 8, n = NU / 2; o > 0; o /= 2, n /= 2) {
+                if (n == 0) m[0] = max(m[0], __shfl_xor_sync(0xffffffffu, m[0], o));
 #pragma unroll
                 for (int k = 0; k < n; ++k) {
                     const bool upper = lane & o;
@@ -564,7 +565,7 @@ struct AnyColumns {
                     m[k] = max(keep, __shfl_xor_sync(0xffffffffu, give, o));
                 }
             }
-            return max(m[0], __shfl_xor_sync(0xffffffffu, m[0], 1));
+            return m[0];
         }
     }
     // The row's codes and scale bytes; PLAIN: all columns are there and all blocks are finite.
@@ -589,7 +590,7 @@ struct AnyColumns {
     __device__ __forceinline__ void keep(uint8_t* q, uint8_t* sc, int warp, int blocks, bool e4m3, const F2* v) const {
         const uint32_t e = scale_byte(__uint_as_float(block_most(v)), e4m3);
         const int block = warp * kWarpBlocks + block_of_lane();
-        if ((W == 1 ? threadIdx.x % 32 < 16 : threadIdx.x % 2 == 0) && block < blocks) sc[block] = (uint8_t)e;
+        if ((W == 1 ? threadIdx.x % 32 < E : threadIdx.x % kLanes == 0) && block < blocks) sc[block] = (uint8_t)e;
         const float inv = e == 255u ? 0.f : inverse_scale(e);
         if (__all_sync(0xffffffffu, full && e != 255u)) {
             if (e4m3) store_codes<true, true>(q, v, inv);
@@ -665,10 +666,10 @@ struct AnyColumns {
         const F2 minus = f2(-mean);
         if (full) {
 #pragma unroll
-            for (int j = 0; j < kAnyElems / 2; ++j) v[j] = f2_add(v[j], minus);
+            for (int j = 0; j < E / 2; ++j) v[j] = f2_add(v[j], minus);
         } else {
 #pragma unroll
-            for (int j = 0; j < kAnyElems / 2; ++j)
+            for (int j = 0; j < E / 2; ++j)
                 v[j] = f2_add(v[j], W == 2 ? f2(j < count ? -mean : 0.f) : f2(2 * j < count ? -mean : 0.f, 2 * j + 1 < count ? -mean : 0.f));
         }
     }
@@ -686,17 +687,16 @@ struct AnyColumns {
     }
 };
 
-template <typename T, int W, int THREADS, bool KEEP>
+template <typename T, int W, int E, int THREADS, bool KEEP>
 __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1)
 norm_forward_any_kernel(NormArgs a) {
-    constexpr int E = kAnyElems;
     extern __shared__ char pieces[];
     __shared__ __align__(16) float shares[THREADS / 64][4][kShare];
     for (int i = threadIdx.x; i < (int)(sizeof(shares) / 4); i += blockDim.x) (&shares[0][0][0])[i] = 0.f;
     __syncthreads();
     grid_dependency_wait();
     const RingPlace p(a.group, a.rows, a.step);
-    const AnyColumns<W> mine(p.t, (int)a.d);
+    const AnyColumns<W, E> mine(p.t, (int)a.d);
     const PieceRing<T> ring(a.x, a.d, a.ldx, a.rows, pieces + p.group * kAnyStages * a.pitch, a.pitch);
 #pragma unroll
     for (int s = 0; s < kAnyStages - 1; ++s) {
@@ -745,10 +745,9 @@ norm_forward_any_kernel(NormArgs a) {
     }
 }
 
-template <typename T, int W, bool KEPT>
+template <typename T, int W, int E, bool KEPT>
 __global__ void __launch_bounds__(kAnyThreads)
 norm_backward_any_kernel(NormArgs a) {
-    constexpr int E = kAnyElems;
     extern __shared__ char pieces[];                      // [group][stage]: dy, then of all groups x or codes
     __shared__ __align__(16) float2 shares[kAnyThreads / 64][2][kShare];
     for (int i = threadIdx.x; i < (int)(sizeof(shares) / 8); i += blockDim.x) (&shares[0][0][0])[i] = make_float2(0.f, 0.f);
@@ -756,7 +755,7 @@ norm_backward_any_kernel(NormArgs a) {
     grid_dependency_wait();
     const RingPlace p(a.group, a.rows, a.step);
     const int G = a.group, d = (int)a.d, per_block = blockDim.x / G;
-    const AnyColumns<W> mine(p.t, d);
+    const AnyColumns<W, E> mine(p.t, d);
     using S = typename std::conditional<KEPT, uint8_t, T>::type;
     char* second = pieces + per_block * kAnyStages * a.pitch;
     const PieceRing<T> ring(a.dy, a.d, a.lddy, a.rows, pieces + p.group * kAnyStages * a.pitch, a.pitch);
@@ -774,7 +773,7 @@ norm_backward_any_kernel(NormArgs a) {
     float2* share = &shares[p.warps > 1 ? p.group : 0][0][0];
     int stage = 0, row = (int)p.row;
     // what a row needs beside the rings is loaded one row ahead
-    const int block = p.warp * AnyColumns<W>::kWarpBlocks + AnyColumns<W>::block_of_lane();
+    const int block = p.warp * AnyColumns<W, E>::kWarpBlocks + AnyColumns<W, E>::block_of_lane();
     float rstd_next = 0.f, mean_next = 0.f;
     uint32_t scale_next = 0;
     auto ahead = [&](int r, bool live) {
@@ -1044,6 +1043,14 @@ static cudaError_t allow_shared(const void* kernel, size_t bytes, int dev) {
     return e;
 }
 
+// Columns of a thread for rows of any alignment: fewer where a row is less than a warp's worth of them.
+template <typename F>
+static auto any_elements(int64_t d, F f) {
+    if (d <= 32 * 4) return f(std::integral_constant<int, 4>{});
+    if (d <= 32 * 8) return f(std::integral_constant<int, 8>{});
+    return f(std::integral_constant<int, kAnyElems>{});
+}
+
 struct NormLaunch {
     b200_stream_t st;
     NormArgs a;
@@ -1097,8 +1104,13 @@ static cudaError_t run_forward(b200_stream_t st, NormArgs a, int v) {
             auto run = [&](auto kernel) { const cudaError_t e = l.plan(kernel, per, bytes); return e == cudaSuccess ? l.go(kernel) : e; };
             auto width = [&](auto w) {
                 constexpr int W = decltype(w)::value;
-                if (a.group <= 256) return a.q ? run(norm_forward_any_kernel<T, W, 256, true>) : run(norm_forward_any_kernel<T, W, 256, false>);
-                return a.q ? run(norm_forward_any_kernel<T, W, 512, true>) : run(norm_forward_any_kernel<T, W, 512, false>);
+                return any_elements(a.d, [&](auto e) {
+                    constexpr int E = decltype(e)::value;
+                    if constexpr (E == kAnyElems) {
+                        if (a.group > 256) return a.q ? run(norm_forward_any_kernel<T, W, E, 512, true>) : run(norm_forward_any_kernel<T, W, E, 512, false>);
+                    }
+                    return a.q ? run(norm_forward_any_kernel<T, W, E, 256, true>) : run(norm_forward_any_kernel<T, W, E, 256, false>);
+                });
             };
             if constexpr (sizeof(T) == 2) { if (a.units2) return width(std::integral_constant<int, 2>{}); }
             return width(std::integral_constant<int, 1>{});
@@ -1191,10 +1203,13 @@ static int32_t run_backward(b200_stream_t st, NormArgs a, int v, void* dgamma, v
             B200_CUDA(l.go(kernel));
             return B200_OK;
         };
-        if constexpr (k16) {
-            if (a.units2) B200_TRY(a.q ? run(norm_backward_any_kernel<T, 2, true>) : run(norm_backward_any_kernel<T, 2, false>));
-        }
-        if (!a.units2) B200_TRY(a.q ? run(norm_backward_any_kernel<T, 1, true>) : run(norm_backward_any_kernel<T, 1, false>));
+        B200_TRY(any_elements(a.d, [&](auto e) -> int32_t {
+            constexpr int E = decltype(e)::value;
+            if constexpr (k16) {
+                if (a.units2) return a.q ? run(norm_backward_any_kernel<T, 2, E, true>) : run(norm_backward_any_kernel<T, 2, E, false>);
+            }
+            return a.q ? run(norm_backward_any_kernel<T, 1, E, true>) : run(norm_backward_any_kernel<T, 1, E, false>);
+        }));
     } else {
         const int64_t tiles = (a.d + 31) / 32;
         int64_t n = (int64_t)sm_count(st->dev) * 8 / tiles;

@@ -325,3 +325,25 @@ def test_rows_over_several_streams(gpu):
         gpu.layernorm_(Z, Y, stream=b)
         gpu.layernorm_(W, Z, stream=a)
         assert bits_equal(W.to_host(), want)
+
+
+NARROW = [(34, 40), (66, 50), (70, 9), (101, 300), (127, 33), (129, 64), (130, 17), (201, 41), (202, 40), (255, 7), (257, 5), (258, 30),
+          (390, 20), (511, 9), (514, 11), (1026, 9), (1536, 40), (2046, 5), (3000, 7), (4094, 4), (4095, 3), (6144, 9), (6145, 2), (8190, 2)]
+
+
+def uneven_rows(rng, d, n, t):
+    """Rows whose blocks of 32 differ in magnitude, so that no block's scale fits its neighbour."""
+    x = rng.standard_normal((d, n)) * np.ldexp(1.0, (np.arange(d) // 32 * 5 % 9) - 4)[:, None] + 0.25
+    return x.astype(t)
+
+
+@pytest.mark.parametrize("dtype", list(ref.TYPES))
+def test_rows_of_many_widths(gpu, dtype, monkeypatch):
+    """Widths on either side of what a thread, a warp and a block of threads hold, at every alignment of 16-bit rows."""
+    import sys
+    here = sys.modules[__name__]
+    monkeypatch.setattr(here, "SHAPES", NARROW)
+    monkeypatch.setattr(here, "rows", uneven_rows)
+    test_forward_and_gradient(gpu, dtype, True)
+    for form in ("int8", "e4m3"):
+        test_checkpoint(gpu, dtype, form)
