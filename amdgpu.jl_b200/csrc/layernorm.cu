@@ -54,11 +54,15 @@ __device__ __forceinline__ float lane_sum(float v, int width) {
 // 66 us; waiting for each row in turn the gradient takes 120 us.  A register spilled inside the loop costs
 // more than a second pass over it (20 bytes: 69 -> 84 us).
 //
-// FULL: rows that fill every thread of whole warps (d = group * E).  A warp's vectors lie side by side there,
-// so that a thread's steps through a row are known at compile time, and nothing is predicated: 8192 x 5120
-// BFloat16 forward with the 8-bit rows 41 us (44 without), gradient from them 50 us (56), 8192 x 6144 Float16
-// 46 (55) and 55 (61) us, 8192 x 8192 gradient 79 (84) us; 16384 x 4096 forward with the 8-bit rows 63 (61) us.
+// Rows that fill every thread of whole warps (d = group * E) lie warp by warp, so that a thread's steps
+// through a row are known at compile time, and nothing is predicated: 8192 x 5120 BFloat16 forward with the
+// 8-bit rows 41 us (44 without), gradient from them 50 us (56), 8192 x 6144 Float16 46 (55) and 55 (61) us,
+// 8192 x 8192 gradient 79 (84) us; 16384 x 4096 forward with the 8-bit rows 63 (61) us.  The steps alone, for
+// rows that leave threads empty: 16000 x 2624 forward with the 8-bit rows 45 us (47).
 
+// How a row lies over its group: neighbouring vectors over all threads; over the threads of each warp, so
+// that steps are known at compile time; the same with every thread filled, so that nothing is predicated.
+enum { kOverGroup = 0, kOverWarps = 1, kFilled = 2 };
 enum { kAsIs = 0 };                     // form of the rows kept for the gradient: as they are, kInt8, kE4M3
 
 struct GroupBarrier {
@@ -163,7 +167,7 @@ __device__ __forceinline__ void load_params2(const NormArgs& a, const void* p, i
 }
 
 // Two passes over the row in registers: the mean first, then the squares about it.
-template <typename T, int E, int STAGES, int THREADS, int KEEP, bool FULL>
+template <typename T, int E, int STAGES, int THREADS, int KEEP, int FORM>
 __global__ void __launch_bounds__(THREADS)
 norm_forward_ring_kernel(NormArgs a) {
     constexpr int V = 16 / (int)sizeof(T), NV = E / V, SLOT = NV * THREADS;
@@ -173,10 +177,10 @@ norm_forward_ring_kernel(NormArgs a) {
     __syncthreads();
     grid_dependency_wait();
     const RingPlace p(a.group, a.rows, a.step);
-    const int S = FULL ? 32 : a.group, t = FULL ? p.warp * (32 * NV) + p.lane : p.t, nvec = (int)(a.d / V);
+    const int S = FORM ? 32 : a.group, t = FORM ? p.warp * (32 * NV) + p.lane : p.t, nvec = (int)(a.d / V);
     bool in[NV];
 #pragma unroll
-    for (int k = 0; k < NV; ++k) in[k] = FULL || t + k * S < nvec;
+    for (int k = 0; k < NV; ++k) in[k] = FORM == kFilled || t + k * S < nvec;
     const T* src = reinterpret_cast<const T*>(a.x) + p.row * a.ldx + (int64_t)t * V;      // next row to fetch
     T* dst = reinterpret_cast<T*>(a.y) + p.row * a.ldy + (int64_t)t * V;
     uint8_t* dst_q = a.q + p.row * a.d + t * V;
@@ -209,7 +213,7 @@ norm_forward_ring_kernel(NormArgs a) {
     float* share = &shares[p.warps > 1 ? p.group : 0][0][0];
     int64_t row = p.row;
     for (int it = 0; it < p.walk; ++it, row += a.step) {
-        const bool live = FULL || it < p.mine;
+        const bool live = FORM || it < p.mine;
         cp_async_wait<STAGES - 2>();
         F2 v[E / 2];
         F2 sum2 = f2(0.f);
@@ -267,7 +271,7 @@ norm_forward_ring_kernel(NormArgs a) {
 
 // dx needs the row again after its sums: g gamma and h stay in registers (HOLD), or the row is read out
 // of the ring a second time and the registers are for the column sums of more columns.
-template <typename T, int E, int STAGES, int THREADS, int KEPT, bool HOLD, bool FULL>
+template <typename T, int E, int STAGES, int THREADS, int KEPT, bool HOLD, int FORM>
 __global__ void __launch_bounds__(THREADS)
 norm_backward_ring_kernel(NormArgs a) {
     constexpr int V = 16 / (int)sizeof(T), NV = E / V, SLOT = NV * THREADS;
@@ -278,10 +282,10 @@ norm_backward_ring_kernel(NormArgs a) {
     __syncthreads();
     grid_dependency_wait();
     const RingPlace p(a.group, a.rows, a.step);
-    const int S = FULL ? 32 : a.group, t = FULL ? p.warp * (32 * NV) + p.lane : p.t, nvec = (int)(a.d / V), per_block = blockDim.x / a.group;
+    const int S = FORM ? 32 : a.group, t = FORM ? p.warp * (32 * NV) + p.lane : p.t, nvec = (int)(a.d / V), per_block = blockDim.x / a.group;
     bool in[NV];
 #pragma unroll
-    for (int k = 0; k < NV; ++k) in[k] = FULL || t + k * S < nvec;
+    for (int k = 0; k < NV; ++k) in[k] = FORM == kFilled || t + k * S < nvec;
     const T* src = reinterpret_cast<const T*>(a.dy) + p.row * a.lddy + (int64_t)t * V;    // next row to fetch
     const T* src_x = reinterpret_cast<const T*>(a.x) + p.row * a.ldx + (int64_t)t * V;
     const uint8_t* src_q = a.q + p.row * a.d + (int64_t)t * V;
@@ -318,7 +322,7 @@ norm_backward_ring_kernel(NormArgs a) {
     // gamma lies in shared memory, [vector][quarter][thread], where threads' vectors lie side by side: the
     // registers are taken
     float4* gammas = reinterpret_cast<float4*>(reinterpret_cast<char*>(ring) + (size_t)STAGES * SLOT * (16 + (KEPT ? V : 16))) +
-                     (FULL ? p.warp * (32 * E / 4) + p.lane : t);
+                     (FORM ? p.warp * (32 * E / 4) + p.lane : t);
     if (p.group == 0) {
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
@@ -357,7 +361,7 @@ norm_backward_ring_kernel(NormArgs a) {
     int slot = 0, free_slot = (STAGES - 1) * SLOT;
     float2* share = &shares[p.warps > 1 ? p.group : 0][0][0];
     for (int it = 0; it < p.walk; ++it, row += (int)a.step) {
-        const bool live = it < p.mine;                    // FULL: always; without the branch the loads below move about and spill
+        const bool live = it < p.mine;                    // whole warps: always; without the branch the loads below move about and spill
         const float rstd = rstd_next;
         const F2 r2 = f2(rstd), minus = f2(-mean_next);
         cp_async_wait<STAGES - 2>();
@@ -1029,8 +1033,15 @@ static int norm_vector(const NormArgs& a, int32_t dtype, bool aligned) {
     const int v = dtype == B200_F32 ? 4 : 8;
     return aligned && a.d % v == 0 && a.rows <= 0x3fffffff ? v : 1;    // the ring kernels count rows in 32 bits
 }
-// Whole warps that have all their columns: nothing is predicated.
-static bool full_rows(const NormArgs& a, int e) { return a.group % 32 == 0 && a.d == (int64_t)a.group * e; }
+// f(constant): how a row lies over its group.
+template <bool WARPS, typename F>
+static auto by_form(const NormArgs& a, int e, F f) {
+    if (a.group % 32 == 0) {
+        if (a.d == (int64_t)a.group * e) return f(std::integral_constant<int, kFilled>{});
+        if constexpr (WARPS) return f(std::integral_constant<int, kOverWarps>{});
+    }
+    return f(std::integral_constant<int, kOverGroup>{});
+}
 // Dynamic shared memory that with the static one may pass 48 KB has to be allowed once per kernel and device.
 static cudaError_t allow_shared(const void* kernel, size_t bytes, int dev) {
     if (bytes <= 32 * 1024) return cudaSuccess;
@@ -1081,11 +1092,11 @@ static cudaError_t forward_ring(b200_stream_t st, const NormArgs& a) {
     const size_t bytes = (size_t)STAGES * (E * sizeof(T)) * THREADS;
     auto run = [&](auto kernel) { const cudaError_t e = l.plan(kernel, per, bytes); return e == cudaSuccess ? l.go(kernel) : e; };
     auto form = [&](auto full) {
-        constexpr bool FULL = decltype(full)::value;
-        if (!a.q) return run(norm_forward_ring_kernel<T, E, STAGES, THREADS, kAsIs, FULL>);
-        return a.e4m3 ? run(norm_forward_ring_kernel<T, E, STAGES, THREADS, kE4M3, FULL>) : run(norm_forward_ring_kernel<T, E, STAGES, THREADS, kInt8, FULL>);
+        constexpr int FORM = decltype(full)::value;
+        if (!a.q) return run(norm_forward_ring_kernel<T, E, STAGES, THREADS, kAsIs, FORM>);
+        return a.e4m3 ? run(norm_forward_ring_kernel<T, E, STAGES, THREADS, kE4M3, FORM>) : run(norm_forward_ring_kernel<T, E, STAGES, THREADS, kInt8, FORM>);
     };
-    return full_rows(a, E) ? form(std::true_type{}) : form(std::false_type{});
+    return by_form<true>(a, E, form);
 }
 template <typename T>
 static cudaError_t run_forward(b200_stream_t st, NormArgs a, int v) {
@@ -1133,7 +1144,9 @@ static int32_t backward_ring(NormLaunch& l, F space) {
         B200_CUDA(l.go(kernel));
         return B200_OK;
     };
-    return full_rows(l.a, E) ? run(norm_backward_ring_kernel<T, E, STAGES, THREADS, KEPT, HOLD, true>) : run(norm_backward_ring_kernel<T, E, STAGES, THREADS, KEPT, HOLD, false>);
+    // with 32 columns a thread's registers are all taken, and predicates over fixed steps cost more than the
+    // steps (16000 x 2624 BFloat16 54 -> 58 us)
+    return by_form<E == 16>(l.a, E, [&](auto form) { return run(norm_backward_ring_kernel<T, E, STAGES, THREADS, KEPT, HOLD, decltype(form)::value>); });
 }
 
 // Workspace of one call.  Outside a capture it is the stream's scratch; inside one the graph gets an
