@@ -85,7 +85,10 @@ __device__ __forceinline__ int turn_at(int i, int half) {
 }
 
 // `group` threads (whole warps) per token; the 32/V lanes of a block of 32 are neighbours.  A thread's first
-// vectors are on their way while the slot is looked at and the angles are worked out.
+// vectors are on their way while the slot is looked at and the angles are worked out.  Bound by latency: a
+// block waits for its slots, then for its angles, once each; looking at slots and angles side by side came out
+// the same.  One B200, 8192 tokens of 8 heads of 128, BFloat16 to e4m3 with the claims settled: 23 us, 17 us
+// without turning (51 MB: 8 us).
 template <typename T, int V, int F, int TURN>
 __global__ void __launch_bounds__(256, TURN == kTurnHalf ? 5 : 1)
 cache_write_kernel(CacheArgs a) {
@@ -216,7 +219,8 @@ cache_write_kernel(CacheArgs a) {
 
 // A thread keeps its vector of a token - side, head and place are worked out once - and walks over the
 // tokens of the block's tile, kReadUnroll at a time: their pages are looked up together, then their codes
-// are loaded together.
+// are loaded together.  Bound by HBM.  One B200, 8 contexts of up to 16384 tokens of 8 heads of 128, e4m3 to
+// BFloat16: 80 us (6.0 TB/s of codes read and rows written), with a thread per vector and token 137 us.
 constexpr int kReadUnroll = 4;
 
 template <typename T, int V, int F>

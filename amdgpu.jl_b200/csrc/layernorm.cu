@@ -474,6 +474,12 @@ norm_backward_ring_kernel(NormArgs a) {
 // through the ring, and a thread picks its columns t, t + group, ... out of them one by one, so its gamma and
 // its column sums stay its own whatever a row's offset.  The pieces are shared by a group: one more barrier
 // per row.  Pieces that reach past the first or the last byte of the array are copied element by element.
+// Bound by instruction issue (an access per element, and a row's fixed work), so a thread has fewer columns
+// where rows are narrow, a block's scale is worked out by one lane and handed to the others, and whole warps
+// skip the predicates.  One B200, 16384 x 4095 BFloat16 (4096: in brackets): forward 90 us (48), with the
+// 8-bit rows 151 us (63), gradient 118 us (69), from the 8-bit rows 124 us (66); 200000 x 101 Float16 68, 97,
+// 78 and 82 us (16 columns per thread: 106, 204, 136 and 145 us).  With a block per row that reads it three
+// times out of L2, as longer rows still go, 16384 x 4095 takes 266 us forward and as long for the gradient.
 constexpr int kAnyElems = 16;
 constexpr int kAnyStages = 3;
 constexpr int kAnyThreads = 512;
@@ -859,7 +865,7 @@ norm_backward_any_kernel(NormArgs a) {
     }
 }
 
-// Sums the partials: 4 W columns per block (W lanes of four), 1024 / W strands of partials, joined in a
+// Sums the partials (a few MB, out of L2): 4 W columns per block (W lanes of four), 1024 / W strands of partials, joined in a
 // fixed order.  VEC: d is a multiple of 4, so four columns are one access.
 template <bool VEC>
 __global__ void __launch_bounds__(1024)
