@@ -85,10 +85,10 @@ __device__ __forceinline__ int turn_at(int i, int half) {
 }
 
 // `group` threads (whole warps) per token; the 32/V lanes of a block of 32 are neighbours.  A thread's first
-// vectors are on their way while the slot is looked at and the angles are worked out.  Bound by latency: a
-// block waits for its slots, then for its angles, once each; looking at slots and angles side by side came out
-// the same.  One B200, 8192 tokens of 8 heads of 128, BFloat16 to e4m3 with the claims settled: 23 us, 17 us
-// without turning (51 MB: 8 us).
+// vectors are on their way while the slot is looked at and the angles are worked out.  Bound by latency
+// and instruction issue: a token waits for its slot, then for its angles; working out both at once and fetching
+// vectors ahead came out the same.  One B200, BFloat16 to e4m3, 8 heads of 128: 8192 tokens 19 us with the
+// claims settled (51 MB: 8 us), 32768 tokens 60 us (3.4 TB/s), 47 us without turning.
 template <typename T, int V, int F, int TURN>
 __global__ void __launch_bounds__(256, TURN == kTurnHalf ? 5 : 1)
 cache_write_kernel(CacheArgs a) {
@@ -137,7 +137,8 @@ cache_write_kernel(CacheArgs a) {
         }
         where[group] = w;
     }
-    __syncthreads();
+    if (G > 32) __syncthreads();
+    else __syncwarp();
     const int2 w = where[group];
     if (w.x >= 0) {
         // of several tokens with one slot the last is kept, as if they were written in turn
@@ -155,7 +156,8 @@ cache_write_kernel(CacheArgs a) {
             }
         }
     }
-    __syncthreads();
+    if (G > 32) __syncthreads();
+    else __syncwarp();
     const bool write = w.x >= 0 && !lost[group];
     for (int base = 0;;) {
         const CacheSide& side = c.key ? a.k : a.v;
@@ -427,8 +429,13 @@ extern "C" int32_t b200_cache_write(b200_stream_t st, const b200_tensor* KQ, con
         s->units = per * a.heads;
         s->per_head = FastDiv((uint32_t)per);
     }
+    // few tokens: a thread per vector; many: four vectors to a thread, so that there are fewer to look at slots and
+    // angles and a token mostly is one warp, with no barrier (32768 tokens of 8 heads of 128: 60 us, one
+    // vector each 84)
+    const int units = a.k.units + a.v.units, per_thread = a.tokens > kScanTokens ? 4 : 1;
     a.group = 32;
-    while (a.group < 256 && a.group < a.k.units + a.v.units) a.group *= 2;
+    auto angles = [&] { return (size_t)(256 / a.group) * (a.rot / 2) * sizeof(float2); };
+    while (a.group < 256 && (a.group * per_thread < units || angles() > 32 * 1024)) a.group *= 2;
     const int per_block = 256 / a.group;
     void* temp = nullptr;
     if (a.tokens > kScanTokens && a.nslots > 0) {
@@ -442,7 +449,7 @@ extern "C" int32_t b200_cache_write(b200_stream_t st, const b200_tensor* KQ, con
         B200_CUDA(cudaMemsetAsync(p, 0, (size_t)a.nslots * 4, st->s));
         B200_CUDA(launch_overlapped(cache_claim_kernel, (unsigned)((a.tokens + 255) / 256), 256u, 0, st->s, a));
     }
-    const size_t smem = (size_t)per_block * (a.rot / 2) * sizeof(float2);
+    const size_t smem = angles();
     const unsigned grid = (unsigned)((a.tokens + per_block - 1) / per_block);
     B200_CUDA(by_row_type(dtype, v, [&](auto t, auto w) {
         using T = decltype(t);

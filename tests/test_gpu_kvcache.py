@@ -313,3 +313,29 @@ def test_strided_indices_and_value_heads(gpu):
                 l = np.arange(m)
                 row = (np.array(table)[l // 8] - 1) * 8 + l % 8
                 assert np.array_equal(h[:, :, :m, b], full[:, :, row]) and not h[:, :, m:, b].any()
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_many_tokens_of_many_shapes(gpu, layout):
+    """More tokens than are looked through one by one, with heads that take part of a warp, a warp, and several:
+    the slots get what a call with few tokens writes there."""
+    rng = np.random.default_rng(23)
+    half, single = np.dtype(np.float16), np.dtype(np.float32)
+    for d, dv, heads, t in ((32, 32, 1, ref.BF16), (72, 72, 3, half), (128, 64, 8, ref.BF16), (256, 256, 9, ref.BF16), (64, 64, 2, single),
+                            (33, 40, 2, half), (1984, 32, 1, ref.BF16), (8192, 16, 1, half)):
+        n, pages = (2500, 40) if d < 1000 else (2050, 33)
+        K, V = (rng.standard_normal((k, heads, n)).astype(t) for k in (d, dv))
+        slots = rng.permutation(64 * pages)[:n] + 1
+        slots[rng.integers(0, n, 50)] = slots[rng.integers(0, n, 50)]
+        slots[rng.integers(0, n, 20)] = 0
+        positions = rng.integers(-10, 1 << 20, n)
+        plan = gpu.rotary_plan(2 * (d // 3), layout=layout)
+        one, many = (gpu.quantized_cache(d, heads, 64, pages, "e4m3", value_dim=dv) for _ in range(2))
+        up = gpu.ROCArray.from_host
+        gpu.cache_write_(many, up(K), up(V), up(slots), rotary=plan, positions=up(positions))
+        for i in range(0, n, 1000):
+            p = slice(i, i + 1000)
+            gpu.cache_write_(one, up(np.asfortranarray(K[:, :, p])), up(np.asfortranarray(V[:, :, p])), up(slots[p]), rotary=plan, positions=up(positions[p]))
+        gpu.synchronize()
+        for a, b in zip(one._arrays(), many._arrays()):
+            assert np.array_equal(a.to_host(), b.to_host()), (d, heads)
