@@ -36,13 +36,17 @@ struct CacheArgs {
 // the later slots.
 constexpr int64_t kScanTokens = 2048;
 
+// Twice per call: first the words of the call's own slots are cleared (a cache may have many more), then claimed.
+template <bool CLEAR>
 __global__ void __launch_bounds__(256)
 cache_claim_kernel(CacheArgs a) {
     grid_dependency_wait();
     const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (t >= a.tokens) return;
     const int64_t slot = load_int(a.slots, a.slots_wide, t * a.islots);
-    if (slot >= 1 && slot <= a.nslots) atomicMax(a.owner + slot - 1, (uint32_t)t + 1u);
+    if (slot < 1 || slot > a.nslots) return;
+    if constexpr (CLEAR) a.owner[slot - 1] = 0;
+    else atomicMax(a.owner + slot - 1, (uint32_t)t + 1u);
 }
 
 // V elements at `p`: 32 bytes are one access where `wide` says that they are aligned.
@@ -446,8 +450,8 @@ extern "C" int32_t b200_cache_write(b200_stream_t st, const b200_tensor* KQ, con
         if (cap == cudaStreamCaptureStatusNone) B200_TRY(scratch(st, (size_t)a.nslots * 4, &p));
         else { B200_TRY(b200_malloc_async(&temp, (size_t)a.nslots * 4, st)); p = temp; }
         a.owner = reinterpret_cast<uint32_t*>(p);
-        B200_CUDA(cudaMemsetAsync(p, 0, (size_t)a.nslots * 4, st->s));
-        B200_CUDA(launch_overlapped(cache_claim_kernel, (unsigned)((a.tokens + 255) / 256), 256u, 0, st->s, a));
+        B200_CUDA(launch_overlapped(cache_claim_kernel<true>, (unsigned)((a.tokens + 255) / 256), 256u, 0, st->s, a));
+        B200_CUDA(launch_overlapped(cache_claim_kernel<false>, (unsigned)((a.tokens + 255) / 256), 256u, 0, st->s, a));
     }
     const size_t smem = angles();
     const unsigned grid = (unsigned)((a.tokens + per_block - 1) / per_block);
