@@ -91,8 +91,8 @@ __device__ __forceinline__ int turn_at(int i, int half) {
 // `group` threads (whole warps) per token; the 32/V lanes of a block of 32 are neighbours.  A thread's first
 // vectors are on their way while the slot is looked at and the angles are worked out.  Bound by latency
 // and instruction issue: a token waits for its slot, then for its angles; working out both at once and fetching
-// vectors ahead came out the same.  One B200, BFloat16 to e4m3, 8 heads of 128: 8192 tokens 19 us with the
-// claims settled (51 MB: 8 us), 32768 tokens 60 us (3.4 TB/s), 47 us without turning.
+// vectors ahead came out the same.  One B200, BFloat16 to e4m3, 8 heads of 128: 8192 tokens 17 us with the
+// claims settled (51 MB: 8 us), 32768 tokens 58 us (3.5 TB/s), 44 us without turning.
 template <typename T, int V, int F, int TURN>
 __global__ void __launch_bounds__(256, TURN == kTurnHalf ? 5 : 1)
 cache_write_kernel(CacheArgs a) {
