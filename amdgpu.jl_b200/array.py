@@ -98,21 +98,28 @@ def with_managed(stream: Stream, *arrays) -> Stream:
     return stream
 
 
+def check_device(stream: Stream, a: "ROCArray") -> None:
+    """Refuses an array whose memory lies on another device than the stream's.  The stream that used it
+    last says nothing about that: after a copy between devices it is the destination's."""
+    if a.buf.device != stream.device:
+        raise ValueError(f"an array of device {a.buf.device} cannot be used on a stream of device {stream.device}")
+
+
 def on_stream(stream: Stream, *arrays) -> list:
     """:func:`with_managed` for operators that refuse arrays of another device than the stream's; returns
     references to the arrays' descriptors, in their order (``None`` stays).  One walk over the arrays:
     a call on few elements is as long as its host side."""
-    refs = []
+    refs, device = [], stream.device
     for a in arrays:
         if a is None:
             refs.append(None)
             continue
         b = a.buf
+        if b.device != device:
+            check_device(stream, a)
         if b.stream is stream:
             b.dirty = True
         else:
-            if b.device != stream.device:
-                raise ValueError(f"an array of device {b.device} cannot be used on a stream of device {stream.device}")
             b.take_ownership(stream)
         refs.append(a._ref())
     return refs

@@ -8,7 +8,7 @@ from __future__ import annotations
 
 from ._lib import check, lib
 from .array import ROCArray, on_stream
-from .quantization import Quantized8
+from .quantization import Quantized8, copy_on
 from .rotary import RotaryPlan
 from .runtime import Stream, current_stream
 
@@ -53,7 +53,7 @@ def quantized_cache(head_dim: int, heads: int, page_size: int, pages: int, forma
 
 
 def _neighbours(A: ROCArray, st: Stream) -> ROCArray:
-    return A if A._strides is None or A._strides[:1] == (1,) or A.dims[:1] == (1,) else A.copy(st)
+    return A if A._strides is None or A._strides[:1] == (1,) or A.dims[:1] == (1,) else copy_on(A, st)
 
 
 def cache_write_(cache: QuantizedCache, K: ROCArray, V: ROCArray, slots: ROCArray, *, rotary: RotaryPlan | None = None,

@@ -13,7 +13,7 @@ from __future__ import annotations
 import numpy as np
 
 from ._lib import check, lib
-from .array import ROCArray, copyto_, on_stream
+from .array import ROCArray, check_device, copyto_, on_stream
 from .runtime import Stream, current_stream
 
 BLOCK = 32
@@ -41,12 +41,21 @@ def is_rows(A: ROCArray, lead: int) -> bool:
 
 def rows_in(A: ROCArray | None, lead: int, st: Stream) -> ROCArray | None:
     """`A`, or a dense copy where its strides are not those of rows."""
-    return A if A is None or is_rows(A, lead) else A.copy(st)
+    return A if A is None or is_rows(A, lead) else copy_on(A, st)
+
+
+def copy_on(A: ROCArray, st: Stream) -> ROCArray:
+    """A dense copy made by a kernel, so of an array of the stream's own device only."""
+    check_device(st, A)
+    return A.copy(st)
 
 
 def rows_out(A: ROCArray | None, lead: int, st: Stream) -> ROCArray | None:
     """`A`, or a dense stand-in that :func:`rows_back` copies into it."""
-    return A if A is None or is_rows(A, lead) else A.similar(stream=st)
+    if A is None or is_rows(A, lead):
+        return A
+    check_device(st, A)                     # the operator itself sees the stand-in only
+    return A.similar(stream=st)
 
 
 def rows_back(A: ROCArray | None, stand_in: ROCArray | None, st: Stream) -> None:

@@ -13,6 +13,7 @@ import numpy as np
 
 from ._lib import check, lib
 from .array import ROCArray, on_stream
+from .quantization import copy_on
 from .runtime import Stream, current_stream
 
 _LAYOUTS = {"half": 0, "interleaved": 1}
@@ -84,6 +85,6 @@ def rotary_(Y: ROCArray, X: ROCArray, positions: ROCArray, plan: RotaryPlan, *, 
     if Y.dims != X.dims or Y.dtype != X.dtype:
         raise ValueError("rotary: source and destination must have the same size and element type")
     st = stream or current_stream()
-    Xr = X if X._strides is None or X._strides[:1] == (1,) or X.dims[:1] == (1,) else X.copy(st)
+    Xr = X if X._strides is None or X._strides[:1] == (1,) or X.dims[:1] == (1,) else copy_on(X, st)
     check(lib.b200_rotary(st.handle, *on_stream(st, Y, Xr, positions, plan.table), plan._layout, plan.factor, 1 if adjoint else 0))
     return Y

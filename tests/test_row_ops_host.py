@@ -235,3 +235,44 @@ def test_rotary_frequencies(pkg):
             assert math.isclose(a, b / 8, rel_tol=1e-12)
         else:
             assert b / 8 < a < b
+
+
+class _OtherDevice:
+    """A stream of another device than the arrays'."""
+    device, handle = 1, None
+
+
+def test_arrays_of_another_device(pkg):
+    """Refused whatever stream used them last (a copy between devices leaves them with the destination's), and
+    before a stand-in or a dense copy is made of arrays whose strides are not those of rows."""
+    st = _OtherDevice()
+
+    def lent(dtype, dims, strides=None):
+        a = fake(pkg, dtype, dims, strides=strides)
+        a.buf.stream = st                          # as after copyto_ on that stream
+        return a
+    f32 = np.float32
+    for make in (lambda *a, **k: fake(pkg, *a, **k), lent):
+        x, s = make(f32, (32, 6)), make(f32, (32, 6), strides=(6, 1))
+        q = pkg.Quantized8.wrap(make(np.int8, (32, 6)), make(np.uint8, (1, 6)))
+        m, i = make(f32, (6,)), make(np.int32, (3,))
+        h, hs = make(f32, (32, 2, 3)), make(f32, (32, 2, 3), strides=(6, 3, 1))
+        side = pkg.Quantized8.wrap(make(np.int8, (32, 2, 4, 5)), make(np.uint8, (1, 2, 4, 5)))
+        cache = pkg.QuantizedCache(side, side)
+        plan = object.__new__(pkg.RotaryPlan)
+        plan.table, plan.layout, plan._layout, plan.factor = make(np.uint64, (16,)), "half", 0, 1.0
+        for v in (x, s):
+            for call in (lambda: pkg.layernorm_(v, x, stream=st), lambda: pkg.layernorm_(x, v, stream=st),
+                         lambda: pkg.layernorm_backward_(x, v, x, rstd=m, mean=m, stream=st),
+                         lambda: pkg.layernorm_backward_(v, x, q, rstd=m, stream=st),
+                         lambda: pkg.activation_("silu", v, x, stream=st), lambda: pkg.activation_("silu", x, x, v, stream=st),
+                         lambda: pkg.activation_backward_("gelu", v, x, q, stream=st),
+                         lambda: pkg.activation_backward_("gelu", x, x, x, v, dgate=x, stream=st),
+                         lambda: pkg.quantize_(q, v, stream=st), lambda: pkg.dequantize_(v, q, stream=st)):
+                with pytest.raises(ValueError, match="device"):
+                    call()
+        for v in (h, hs):
+            for call in (lambda: pkg.rotary_(h, v, i, plan, stream=st), lambda: pkg.cache_write_(cache, v, h, i, stream=st),
+                         lambda: pkg.cache_write_(cache, h, v, i, stream=st)):
+                with pytest.raises(ValueError, match="device"):
+                    call()
