@@ -379,10 +379,11 @@ __device__ __forceinline__ void decode2(const RawVec<uint8_t, V>& r, uint32_t e,
     }
 }
 // A value near the largest of its type can have been rounded up past it: such blocks saturate.
-// The largest code times 2^(e-127) passes T's largest value only from this e on.
+// The code of largest magnitude (Int8 -128, which no encoder here writes, e4m3 448) times 2^(e-127) passes
+// T's largest value only from this e on.
 template <typename T>
 __device__ __forceinline__ uint32_t saturating_from(bool e4m3) {
-    return sizeof(T) == 2 && Elem<T>::kMax < 1e5f ? (e4m3 ? 135u : 137u) : (e4m3 ? 247u : 249u);
+    return sizeof(T) == 2 && Elem<T>::kMax < 1e5f ? (e4m3 ? 135u : 136u) : (e4m3 ? 247u : 248u);
 }
 // Scales that are far from overflowing anything.
 template <typename T>
@@ -392,7 +393,7 @@ __device__ __forceinline__ void decode_as(const RawVec<uint8_t, V>& r, uint32_t 
     decode<V>(r, e, e4m3, v);
     if (e >= saturating_from<T>(e4m3) && e != 255u) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = fminf(fmaxf(v[i], -Elem<T>::kMax), Elem<T>::kMax);
+        for (int i = 0; i < V; ++i) v[i] = v[i] > Elem<T>::kMax ? Elem<T>::kMax : v[i] < -Elem<T>::kMax ? -Elem<T>::kMax : v[i];     // NaN stays
     }
 }
 

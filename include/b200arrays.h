@@ -294,7 +294,8 @@ int32_t b200_fill_random(b200_stream_t st, const b200_tensor* out, int32_t dist,
  * last block of a row may be shorter.  The scale is 2^(e-127), the smallest such power (e >= 0) that
  * brings the block's largest magnitude to 127 (Int8) or 448 (e4m3); a code is the value over the
  * scale, rounded to nearest even.  A block that holds an infinity or a NaN has e = 255 and reads
- * back as NaN.  Read back into a type too narrow for a value, that value becomes the type's largest. */
+ * back as NaN, as do e4m3's NaN bytes.  Read back into a type too narrow for a value, that value becomes
+ * the type's largest. */
 
 /* Layer norm: the first `lead` dimensions of X are one row, normalised together.
  * Y = (X - m) r gamma + beta, m = mean, r = 1/sqrt(variance + eps) of each row.  gamma and beta hold

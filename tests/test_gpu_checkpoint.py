@@ -216,3 +216,31 @@ def test_blocks_across_vectors(gpu, d, n):
             gpu.activation_("silu", Z, Z, G, checkpoint=qz, gate_checkpoint=qy)
             assert np.array_equal(Z.to_host(), Y.array.to_host(), equal_nan=True) and bits_equal(qz.codes.to_host(), qa.codes.to_host())
             assert bits_equal(qy.scales.to_host(), qb.scales.to_host())
+
+
+@pytest.mark.parametrize("form", ["int8", "e4m3"])
+def test_every_code_at_every_scale(gpu, form):
+    """All 256 codes beside all 256 scale bytes, those that no call of this library writes among them (Int8
+    -128, e4m3 NaN): values past a type's range become its largest, NaN stays NaN."""
+    t8 = np.int8 if form == "int8" else np.uint8
+    e = np.arange(256, dtype=np.uint8)
+    for d in (256, 259):                           # rows of whole vectors, blocks that end inside vectors
+        row = np.resize(np.arange(256, dtype=np.uint8), d).view(t8)
+        codes, scales = np.repeat(row[:, None], 256, 1), np.repeat(e[None], -(-d // 32), 0)
+        q = gpu.Quantized8.wrap(gpu.ROCArray.from_host(codes), gpu.ROCArray.from_host(scales))
+        for t in ref.TYPES.values():
+            want = ref.saturated(ref.restore(codes, scales), t)
+            ref.within(gpu.dequantize(q, t).to_host(), want, 0.0, (d, t))
+            off = gpu.ROCArray(t, d * 256 + 1).view(1, d * 256 + 1).reshape(d, 256)       # an element per lane
+            ref.within(gpu.dequantize_(off, q).to_host(), want, 0.0, (d, t, "off"))
+            side = gpu.Quantized8.wrap(q.codes.reshape(d, 1, 256, 1), q.scales.reshape(-(-d // 32), 1, 256, 1))
+            out = [gpu.zeros(t, (d, 1, 256, 1)) for _ in range(2)]
+            one = gpu.ROCArray.from_host(np.array([[1]], np.int32))
+            gpu.cache_read_(*out, gpu.QuantizedCache(side, side), one, gpu.ROCArray.from_host(np.array([256], np.int32)))
+            ref.within(out[0].to_host().reshape(d, 256), want, 0.0, (d, t, "cache"))
+            # far out the derivatives are 0 and 1
+            far = (np.abs(want) > 1000) | np.isnan(want)
+            slope = np.where(np.isnan(want), np.nan, want > 0)
+            for f in ("silu", "gelu"):
+                got = gpu.activation_backward_(f, gpu.ROCArray(t, (d, 256)), gpu.ones(t, (d, 256)), q).to_host().astype(np.float64)
+                assert np.array_equal(got[far], slope[far], equal_nan=True), (d, t, f)
