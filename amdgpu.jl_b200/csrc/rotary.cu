@@ -6,7 +6,7 @@
 //   y_a = x_a cos - x_b sin,  y_b = x_b cos + x_a sin,  angle = position * frequency[pair]
 //
 // Angles are formed in the kernel from a table of frequencies in 2^-64 turns per position (rowops.cuh):
-// no table of cosines is read, and far positions lose nothing.
+// no table of cosines is read, and a far position loses no more than its multiple of an entry's rounding.
 #include "rowops.cuh"
 
 namespace b200 {

@@ -399,7 +399,8 @@ __device__ __forceinline__ void decode_as(const RawVec<uint8_t, V>& r, uint32_t 
 
 // ---- angles --------------------------------------------------------------------------------------
 // Sine and cosine of a phase counted in 2^-64 turns.  Position times frequency is one wrapping
-// 64-bit product, so an angle is as exact at position 2^31 as at position 1.  The phase is taken to
+// 64-bit product: what a table's entry is off by (2^-65 turns, where it was rounded once) times the
+// position is all that far positions lose, 4e-9 turns at 2^37.  The phase is taken to
 // the nearest quarter turn and the rest, at most pi/4, goes through the Taylor series (terms left
 // out: below 2e-9).
 __device__ __forceinline__ void phase_sincos(uint64_t phase, float factor, float& sn, float& cs) {

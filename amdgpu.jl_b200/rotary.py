@@ -2,11 +2,13 @@
 
 Element-wise over views of the projection's result, where the reference's user writes strided
 broadcasts with tables of sines and cosines (src/broadcast.jl:3-30).  A plan holds the pairs'
-frequencies in 2^-64 turns per position; position times frequency wraps exactly, so far positions
-are as accurate as near ones and no table of angles is read.
+frequencies in 2^-64 turns per position, rounded once; position times frequency wraps exactly, so an
+angle is off by at most 2^-65 turns per position from the frequency's own and no table of angles is
+read.
 """
 from __future__ import annotations
 
+import functools
 import math
 
 import numpy as np
@@ -27,7 +29,9 @@ def rotary_frequencies(rot: int, base: float = 10000.0, scaling: str = "none", s
     "none": base^(-2i/rot).  "linear": those over `stretch` (positions interpolated).  "ntk": base
     times stretch^(rot/(rot-2)).  "yarn" (Peng et al. 2023): pairs that turn more than `beta_fast`
     times over `original_length` positions keep their frequency, those below `beta_slow` are
-    interpolated, those between are mixed in proportion; factor 0.1 ln(stretch) + 1."""
+    interpolated, those between are mixed in proportion; factor 0.1 ln(stretch) + 1.  (Some models
+    mix by the pair's index between two rounded bounds instead: they pass their own frequencies to
+    :class:`RotaryPlan`.)"""
     if rot < 0 or rot % 2:
         raise ValueError("rotary: an even number of elements is turned")
     if scaling not in _SCALINGS:
@@ -48,6 +52,33 @@ def rotary_frequencies(rot: int, base: float = 10000.0, scaling: str = "none", s
     return f, 1.0
 
 
+_PI_BITS = 1280       # a binary64 is below 2^1024: 64 bits of a turn stay right, and 190 more
+
+
+@functools.cache
+def _two_pi() -> int:
+    """2 pi 2^_PI_BITS to a few units, by Machin's formula pi/4 = 4 arctan(1/5) - arctan(1/239)."""
+    one = 1 << (_PI_BITS + 32)
+
+    def arctan(n):
+        term = total = one // n
+        k = 1
+        while term:
+            term //= -n * n
+            k += 2
+            total += term // k
+        return total
+    return (8 * (4 * arctan(5) - arctan(239))) >> 32
+
+
+def _turns(x: float) -> int:
+    """Angle per position in 2^-64 turns, modulo a turn.  In integers: a binary64 quotient would leave a
+    fast pair 53 of the 64 bits, and the position multiplies what it is off by."""
+    n, d = x.as_integer_ratio()
+    n, d = n << (_PI_BITS + 65), d * _two_pi()
+    return (n // d + 1) // 2 % (1 << 64)
+
+
 class RotaryPlan:
     """What :func:`rotary_` and the cache's write keep between calls: the device table (UInt64, one
     entry per pair), the layout of the pairs and the factor on cosine and sine."""
@@ -59,7 +90,7 @@ class RotaryPlan:
             raise ValueError(f"rotary: layout must be one of {sorted(_LAYOUTS)}, not {layout!r}")
         if not all(math.isfinite(x) for x in frequencies) or not math.isfinite(factor):
             raise ValueError("rotary: frequencies and factor must be finite")
-        turns = [round(x / (2.0 * math.pi) * 2.0 ** 64) % (1 << 64) for x in frequencies]
+        turns = [_turns(float(x)) for x in frequencies]
         self.table = ROCArray.from_host(np.array(turns, dtype=np.uint64), stream)
         self.layout, self._layout, self.factor = layout, _LAYOUTS[layout], float(factor)
 

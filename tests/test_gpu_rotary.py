@@ -122,3 +122,22 @@ def test_large_launches(gpu):
         X = gpu.ROCArray.from_host(x)
         got = gpu.rotary_(X.similar(), X, gpu.ROCArray.from_host(pos), gpu.rotary_plan(d)).to_host()
         ref.within(got, ref.turn(x, pos, freq, 1.0, "half"), ref.turn_slack(x, d, 1.0, "half"), (d, heads, n))
+
+
+def test_positions_of_any_size(gpu):
+    """An angle is off by half of 2^-64 turns per position from the frequency as binary64 has it: as exact at
+    2^40 as at 1."""
+    from fractions import Fraction
+    two_pi = Fraction(6283185307179586476925286766559005768394338798750211641949889, 10 ** 60)
+    d = 128
+    freq, _ = gpu.rotary.rotary_frequencies(d, base=500_000.0)
+    plan = gpu.rotary_plan(d, base=500_000.0)
+    pos = np.array([3, 1 << 31, -(1 << 31) - 5, (1 << 36) + 77, 1 << 40, -(1 << 40) - 1], dtype=np.int64)
+    x = np.random.default_rng(1).standard_normal((d, 2, len(pos))).astype(np.float32)
+    got = gpu.rotary_(gpu.ROCArray(np.float32, x.shape), gpu.ROCArray.from_host(x), gpu.ROCArray.from_host(pos), plan).to_host()
+    turns = np.array([[float((Fraction(f) * int(p) / two_pi) % 1) for p in pos] for f in freq])
+    c, s = np.cos(2 * np.pi * turns)[:, None], np.sin(2 * np.pi * turns)[:, None]
+    a, b = x[: d // 2].astype(np.float64), x[d // 2:].astype(np.float64)
+    pair = np.abs(np.concatenate([a, a])) + np.abs(np.concatenate([b, b]))
+    angle = 2 * np.pi * np.abs(pos).astype(np.float64)[None, None] * 2.0 ** -65
+    ref.within(got, np.concatenate([a * c - b * s, b * c + a * s]), ref.turn_slack(x, d, 1.0, "half") + angle * pair)

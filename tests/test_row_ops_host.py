@@ -276,3 +276,37 @@ def test_arrays_of_another_device(pkg):
                          lambda: pkg.cache_write_(cache, h, v, i, stream=st)):
                 with pytest.raises(ValueError, match="device"):
                     call()
+
+
+def test_rotary_table_is_exact(pkg, monkeypatch):
+    """Entries are the frequencies, as binary64 has them, in 2^-64 turns, rounded once: no error but that
+    rounding is multiplied by a position."""
+    from fractions import Fraction
+    from decimal import Decimal, localcontext
+    with localcontext() as ctx:                    # pi by Machin's formula, in decimals
+        ctx.prec = 700
+
+        def arctan(n):
+            term, total, k = Decimal(1) / n, Decimal(0), 0
+            while abs(term) > Decimal(10) ** -690:
+                total += term / (2 * k + 1) * (-1) ** k
+                term /= n * n
+                k += 1
+            return total
+        two_pi = Fraction(8 * (4 * arctan(5) - arctan(239)))
+    tables = []
+
+    class Kept:
+        @staticmethod
+        def from_host(a, stream=None):
+            tables.append(a)
+    monkeypatch.setattr(pkg.rotary, "ROCArray", Kept)
+    sets = [pkg.rotary.rotary_frequencies(128)[0], pkg.rotary.rotary_frequencies(64, base=1e6, scaling="yarn", stretch=8.0, original_length=4096)[0],
+            [0.0, 1.0, -1.0, 2.0 * math.pi, 5e-324, 1e-30, -0.1, 1e22, 1.7976931348623157e308]]
+    for f in sets:
+        pkg.RotaryPlan(f)
+        assert tables[-1].dtype == np.uint64
+        for got, x in zip(tables[-1], f):
+            turns = Fraction(x) / two_pi * (1 << 64)
+            off = (int(got) - turns) % (1 << 64)
+            assert min(off, (1 << 64) - off) <= Fraction(1, 2) + Fraction(1, 1 << 60), x
