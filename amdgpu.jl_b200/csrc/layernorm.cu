@@ -1296,7 +1296,12 @@ extern "C" int32_t b200_layernorm(b200_stream_t st, const b200_tensor* Y, const 
     if (x.d > 0x7fffffff) return fail(B200_TOO_LARGE, "layernorm: rows of at most 2^31-1 elements");
     B200_TRY(enter(st));
     StreamGuard guard(st);
-    if (x.rows == 0 || x.d == 0) return B200_OK;
+    if (x.rows == 0) return B200_OK;
+    if (x.d == 0) {          // moments over no elements
+        for (const b200_tensor* t : {mean, rstd})
+            if (t) B200_TRY(b200_memset_async(t->ptr, 0x7fc00000, 4, (size_t)x.rows, st));
+        return finish(st, "b200_layernorm");
+    }
     NormArgs a{};
     a.x = x.p; a.ldx = x.ld; a.y = y.p; a.ldy = y.ld; a.rows = x.rows; a.d = x.d; a.eps = (float)eps;
     a.gamma = gamma ? gamma->ptr : nullptr;

@@ -300,9 +300,9 @@ int32_t b200_fill_random(b200_stream_t st, const b200_tensor* out, int32_t dist,
 /* Layer norm: the first `lead` dimensions of X are one row, normalised together.
  * Y = (X - m) r gamma + beta, m = mean, r = 1/sqrt(variance + eps) of each row.  gamma and beta hold
  * one value per element of a row, both Float32 or both of X's type; either may be NULL.  mean, rstd:
- * NULL, or Float32, one per row, for the gradient.  Q, S: NULL, or receive the rows (X - m) r in
- * 8 bits (lead must be 1), which the gradient takes instead of X and mean; codes that did not come from
- * here must hold magnitudes below 2^73.  Rows are dense and may be
+ * NULL, or Float32, one per row, for the gradient (NaN for rows of no elements).  Q, S: NULL, or
+ * receive the rows (X - m) r in 8 bits (lead must be 1), which the gradient takes instead of X and
+ * mean; codes that did not come from here must hold magnitudes below 2^73.  Rows are dense and may be
  * any one distance apart. */
 int32_t b200_layernorm(b200_stream_t st, const b200_tensor* Y, const b200_tensor* X, int32_t lead,
                        const b200_tensor* gamma, const b200_tensor* beta, double eps,

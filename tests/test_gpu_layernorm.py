@@ -347,3 +347,12 @@ def test_rows_of_many_widths(gpu, dtype, monkeypatch):
     test_forward_and_gradient(gpu, dtype, True)
     for form in ("int8", "e4m3"):
         test_checkpoint(gpu, dtype, form)
+
+
+def test_moments_of_rows_without_elements(gpu):
+    """0/0, as a mean over nothing is everywhere: what stood in the arrays before does not stay."""
+    for t in ref.TYPES.values():
+        X = gpu.ROCArray(t, (0, 5))
+        M, R = gpu.fill(np.float32(7), 5), gpu.fill(np.float32(7), 5)
+        gpu.layernorm_(X, X, mean=M, rstd=R)
+        assert np.isnan(M.to_host()).all() and np.isnan(R.to_host()).all()
