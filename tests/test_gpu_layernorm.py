@@ -356,3 +356,31 @@ def test_moments_of_rows_without_elements(gpu):
         M, R = gpu.fill(np.float32(7), 5), gpu.fill(np.float32(7), 5)
         gpu.layernorm_(X, X, mean=M, rstd=R)
         assert np.isnan(M.to_host()).all() and np.isnan(R.to_host()).all()
+
+
+@pytest.mark.parametrize("form", ["int8", "e4m3"])
+def test_codes_of_any_alignment(gpu, form):
+    """Checkpoints that are views off 16, 8, 4 and 2 bytes, scale bytes off theirs: the codes are those of an
+    aligned checkpoint, and the gradient is the formula's."""
+    rng = np.random.default_rng(31)
+    for t in ref.TYPES.values():
+        for d, n in ((64, 300), (101, 400), (1000, 30), (1024, 40), (4096, 9), (9002, 3)):
+            x, dy = uneven_rows(rng, d, n, t), rng.standard_normal((d, n)).astype(t)
+            gamma, _ = params(rng, d, t)
+            X, DY, G = (gpu.ROCArray.from_host(a) for a in (x, dy, gamma))
+            want, R = gpu.Quantized8((d, n), form), gpu.ROCArray(np.float32, n)
+            gpu.layernorm_(X.similar(), X, rstd=R, checkpoint=want)
+            # element by element codes may lie beside a rounding's border: sums in another order
+            kept64 = ref.restore(want.codes.to_host(), want.scales.to_host())
+            for off in (1, 2, 4, 8):
+                codes, scales = (Guarded(gpu, a.dtype, a.dims, misalign=off) for a in (want.codes, want.scales))
+                q = gpu.Quantized8.wrap(codes.array, scales.array)
+                gpu.layernorm_(X.similar(), X, rstd=R, checkpoint=q)
+                codes.check((d, n, off)); scales.check((d, n, off))
+                kept = ref.restore(codes.array.to_host(), scales.array.to_host())
+                scale = np.repeat(np.ldexp(1.0, np.maximum(scales.array.to_host(), want.scales.to_host()).astype(int) - 127), 32, 0)[:d]
+                step = scale if form == "int8" else np.maximum(2.0 ** -3 * np.maximum(np.abs(kept), np.abs(kept64)), 2.0 ** -9 * scale)
+                assert (np.abs(kept - kept64) <= step).all(), (d, n, off)
+                DX, DG, DB = gpu.ROCArray(t, (d, n)), gpu.ROCArray(t, d), gpu.ROCArray(t, d)
+                gpu.layernorm_backward_(DX, DY, q, G, rstd=R, dgamma=DG, dbeta=DB)
+                check_backward(kept, R.to_host().astype(np.float64), dy, gamma, DX.to_host(), DG.to_host(), DB.to_host(), 0.0, (d, n, off))
