@@ -33,7 +33,8 @@ struct CacheArgs {
 };
 
 // Tokens above this many settle two claims on one slot through a table instead of by looking through
-// the later slots.
+// the later slots.  The table has a word for every slot of the cache, whatever the call writes: 4 bytes a
+// slot of scratch, which the stream keeps (inside a capture: of an allocation of the graph's own).
 constexpr int64_t kScanTokens = 2048;
 
 // Twice per call: first the words of the call's own slots are cleared (a cache may have many more), then claimed.

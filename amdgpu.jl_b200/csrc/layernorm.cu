@@ -47,9 +47,10 @@ __device__ __forceinline__ float lane_sum(float v, int width) {
 // those, so the ring needs no barrier: a thread waits for its own copies.  Groups run on their own, with a
 // hardware barrier each for their sums, so that some load while others compute and store.
 //
-// With the loads out of the way these kernels are bound by instruction issue, not by HBM: arithmetic goes
-// in pairs (F2), a thread has as many columns as its registers hold, and nothing is predicated but the
-// copies and stores (vectors beyond a row read as zeros).  One B200, 16384 x 4096 BFloat16: forward 48 us
+// With the loads out of the way these kernels are held up by their instructions and by the latency of a
+// row's sums (issue slots 38 to 48 % taken at 10 to 14 warps an SM), not by HBM: arithmetic goes in pairs
+// (F2), a thread has as many columns as its registers hold, and nothing is predicated but the copies and
+// stores (vectors beyond a row read as zeros).  One B200, 16384 x 4096 BFloat16: forward 48 us
 // (5.5 TB/s), with the 8-bit rows written as well 63 us, gradient 69 us (5.8 TB/s), from the 8-bit rows
 // 66 us; waiting for each row in turn the gradient takes 120 us.  A register spilled inside the loop costs
 // more than a second pass over it (20 bytes: 69 -> 84 us).
@@ -474,12 +475,16 @@ norm_backward_ring_kernel(NormArgs a) {
 // through the ring, and a thread picks its columns t, t + group, ... out of them one by one, so its gamma and
 // its column sums stay its own whatever a row's offset.  The pieces are shared by a group: one more barrier
 // per row.  Pieces that reach past the first or the last byte of the array are copied element by element.
-// Bound by instruction issue (an access per element, and a row's fixed work), so a thread has fewer columns
-// where rows are narrow, a block's scale is worked out by one lane and handed to the others, and whole warps
-// skip the predicates.  One B200, 16384 x 4095 BFloat16 (4096: in brackets): forward 90 us (48), with the
+// Instructions are what it takes its time for: a shared-memory load, a conversion and a store per element, and
+// a row's fixed work, 27 a thread and element forward and 32 for the gradient (16384 x 4095 BFloat16; issue
+// slots 60 and 54 % taken at 34 and 25 % of the warps, HBM at 30 and 39 %).  So a thread has fewer columns where
+// rows are narrow, a block's scale is worked out by one lane and handed to the others, and whole warps skip
+// the predicates.  Float32 rows have half the elements per byte and lose little: 16384 x 4095 forward 92 us,
+// gradient 137 us (floors 82 and 123).  One B200, 16384 x 4095 BFloat16 (4096: in brackets): forward 90 us (48), with the
 // 8-bit rows 151 us (63), gradient 118 us (69), from the 8-bit rows 124 us (66); 200000 x 101 Float16 68, 97,
-// 78 and 82 us (16 columns per thread: 106, 204, 136 and 145 us).  With a block per row that reads it three
-// times out of L2, as longer rows still go, 16384 x 4095 takes 266 us forward and as long for the gradient.
+// 78 and 82 us (16 columns per thread: 106, 204, 136 and 145 us).  Rows of up to 512 * 16 = 8192 columns; with
+// a block per row that reads it three times out of L2, as longer ones still go, 16384 x 4095 takes 266 us forward
+// and as long for the gradient.
 constexpr int kAnyElems = 16;
 constexpr int kAnyStages = 3;
 constexpr int kAnyThreads = 512;
@@ -916,7 +921,11 @@ norm_fold_kernel(const float* partial, int64_t npartials, int64_t d, void* dgamm
 }
 
 // ---- rows of any length ---------------------------------------------------------------------------
-// One block per row, element accesses, the row read again for each pass (out of L2).
+// One block per row, element accesses, the row read again for each pass (out of L2): misaligned or odd rows
+// past 8192 columns, Float32 gradients past 8192, everything past 16384.  Four to twelve times the floor:
+// 7456 x 9001 BFloat16 forward 353 us (41), gradient 446 us (61), 2048 x 32768 318 (41) and 443 us (61),
+// with 8-bit rows 442 and 628 us (52 each); Float32 gradient 4096 x 16384 494 us (123), 5000 x 12288 434 us (113).
+// 118 instructions a thread and element forward, issue slots 64 % taken, HBM at 8 %.
 __device__ __forceinline__ float block_sum(float v, float* buf) {
     v = lane_sum(v, 32);
     __syncthreads();

@@ -128,7 +128,9 @@ rotary_kernel(RotaryArgs a) {
 // Vectors of a head whose pairs do not lie vector to vector: rot/2 is no multiple of V (half layout), or
 // the head turns in part (interleaved).  A thread reads its vector at once and, in half
 // layout, the partners one by one; destination and source must be apart, since a vector's partners are
-// other threads' vectors.
+// other threads' vectors.  In half layout both members of a pair work out its angle, and the wait for the
+// partners is what shows among the stalls: 8192 tokens of 64 heads, 26 of 80 turned, BFloat16 65 us (floor 26;
+// interleaved 33), Float32 70 us (51).
 template <typename T, int V, bool HALF>
 __global__ void __launch_bounds__(256)
 rotary_uneven_kernel(RotaryArgs a) {

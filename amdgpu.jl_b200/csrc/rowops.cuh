@@ -189,7 +189,7 @@ __device__ __forceinline__ RawVec<T, V> pack(const float* v) {
 
 // ---- pairs of binary32 ------------------------------------------------------------------------------
 // sm_100 issues one instruction for two neighbouring lanes' worth of binary32 arithmetic; the row
-// kernels are bound by instruction issue once their loads are in flight, so they work in pairs.
+// kernels spend their time on instructions once their loads are in flight, so they work in pairs.
 using F2 = unsigned long long;
 __device__ __forceinline__ F2 f2(float lo, float hi) { F2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi)); return r; }
 __device__ __forceinline__ F2 f2(float both) { return f2(both, both); }

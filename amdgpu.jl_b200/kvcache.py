@@ -61,7 +61,8 @@ def cache_write_(cache: QuantizedCache, K: ROCArray, V: ROCArray, slots: ROCArra
     """Writes the tokens of `K` and `V`, (head size, heads, tokens), to their `slots` (Int32 or Int64,
     one per token).  Slot 0 leaves a token out (a padded batch); of several tokens with one slot the
     last is kept; a slot outside the cache is not written and surfaces as an error at the next
-    synchronisation.  With `rotary` the keys are turned to their `positions` on the way."""
+    synchronisation.  With `rotary` the keys are turned to their `positions` on the way.  More than
+    2048 tokens take 4 bytes per slot of the cache as workspace, which the stream keeps."""
     if (rotary is None) != (positions is None):
         raise ValueError("cache write: a rotary plan and positions belong together")
     st = stream or current_stream()

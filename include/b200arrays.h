@@ -345,7 +345,8 @@ int32_t b200_rotary(b200_stream_t st, const b200_tensor* Y, const b200_tensor* X
  * Write: K, V are (head size, heads, tokens); slots (Int32 or Int64) holds one 1-based slot per token,
  * page-major; slot 0 leaves the token out; of several tokens with one slot the last is kept.  A slot
  * outside the cache latches B200_INVALID_ARG, reported by the next b200_stream_sync, and writes
- * nothing.  positions, table, layout, factor: NULL, or turn the keys on the way (b200_rotary). */
+ * nothing.  A call of more than 2048 tokens takes 4 bytes per slot of the cache as workspace, which the
+ * stream keeps.  positions, table, layout, factor: NULL, or turn the keys on the way (b200_rotary). */
 int32_t b200_cache_write(b200_stream_t st, const b200_tensor* KQ, const b200_tensor* KS,
                          const b200_tensor* VQ, const b200_tensor* VS, const b200_tensor* K,
                          const b200_tensor* V, const b200_tensor* slots, const b200_tensor* positions,
@@ -363,7 +364,10 @@ int32_t b200_cache_read(b200_stream_t st, const b200_tensor* K, const b200_tenso
 /* Every operator above can be captured.  An operator that needs more stream scratch than the
  * stream holds answers B200_UNSUPPORTED inside a capture: run the operation once on that stream
  * first (what @captured does when its first capture fails, src/hip/graph.jl:139-168).  Scratch seen
- * by a capture stays allocated as long as the stream lives.  mode: 0 global, 1 thread local,
+ * by a capture stays allocated as long as the stream lives.  A layer norm gradient with dgamma or
+ * dbeta and a cache write of more than 2048 tokens allocate their workspace inside the graph instead,
+ * so that graphs of one stream may run side by side; CUDA gives such a graph one executable at a time (a
+ * second b200_graph_instantiate fails while the first lives).  mode: 0 global, 1 thread local,
  * 2 relaxed (hipStreamCaptureMode). */
 int32_t b200_graph_capture_begin(b200_stream_t st, int32_t mode);
 /* *out = NULL and an error status when the capture was invalidated */
