@@ -88,9 +88,10 @@ class RotaryPlan:
     def __init__(self, frequencies, layout: str = "half", factor: float = 1.0, stream: Stream | None = None):
         if layout not in _LAYOUTS:
             raise ValueError(f"rotary: layout must be one of {sorted(_LAYOUTS)}, not {layout!r}")
-        if not all(math.isfinite(x) for x in frequencies) or not math.isfinite(factor):
+        frequencies = [float(x) for x in frequencies]
+        if not all(map(math.isfinite, frequencies)) or not math.isfinite(factor):
             raise ValueError("rotary: frequencies and factor must be finite")
-        turns = [_turns(float(x)) for x in frequencies]
+        turns = [_turns(x) for x in frequencies]
         self.table = ROCArray.from_host(np.array(turns, dtype=np.uint64), stream)
         self.layout, self._layout, self.factor = layout, _LAYOUTS[layout], float(factor)
 

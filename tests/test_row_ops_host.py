@@ -310,3 +310,20 @@ def test_rotary_table_is_exact(pkg, monkeypatch):
             turns = Fraction(x) / two_pi * (1 << 64)
             off = (int(got) - turns) % (1 << 64)
             assert min(off, (1 << 64) - off) <= Fraction(1, 2) + Fraction(1, 1 << 60), x
+
+
+def test_rotary_frequencies_of_any_iterable(pkg, monkeypatch):
+    """A generator is gone through once: its frequencies are looked at and kept."""
+    tables = []
+
+    class Kept:
+        @staticmethod
+        def from_host(a, stream=None):
+            tables.append(a)
+    monkeypatch.setattr(pkg.rotary, "ROCArray", Kept)
+    f = pkg.rotary.rotary_frequencies(16)[0]
+    for given in (f, tuple(f), np.array(f), (x for x in f)):
+        pkg.RotaryPlan(given)
+        assert np.array_equal(tables[-1], tables[0]) and len(tables[-1]) == 8
+    with pytest.raises(ValueError, match="finite"):
+        pkg.RotaryPlan(x for x in (1.0, math.inf))
